@@ -507,6 +507,86 @@ size_t sd_norm_gate_backward_scratch_bytes(int64_t rows, int32_t V);
 int sd_norm_gate_forward(const sd_norm_gate_args *args, void *stream);
 int sd_norm_gate_backward(const sd_norm_gate_args *args, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Serving operators (no upstream counterpart): 8-bit projections and token sampling.
+ *
+ * sd_quantize_rows  every row of x in int8 with one FP32 scale: with a = max |x_k| of the row,
+ *                   scale = a / 127 and q_k = 127 x_k / a to the nearest whole number, ties to even.
+ *                   A row of zeros has scale 0; one with an infinity or a NaN has q = 0 and scale NaN.
+ * sd_int8_linear    y[i][j] = x_scale[i] weight_scale[j] sum_k q[i][k] weight[j][k] + bias[j], the sum exact
+ *                   in int32, the rest in FP32, rounded once to the type of y.  x is either int8 (q, with
+ *                   x_scale) or BF16 / FP32, which is quantised first as sd_quantize_rows does.  With swiglu
+ *                   y has N / 2 columns, silu(column j) * (column j + N / 2).
+ *
+ * q and int8 weights and rows start on 16-byte boundaries, their strides are multiples of 16 and at least K
+ * rounded up to 16, and that many bytes of every row are readable (what they hold past K does not matter).
+ * K <= 131072.  sd_int8_linear_scratch_bytes says what a call with these arguments needs for the quantised
+ * rows (0 for int8 rows and where none is needed); scratch is 16-byte aligned.
+ */
+enum { SD_BF16 = 0, SD_F32 = 1, SD_I8 = 2 };
+
+typedef struct {
+    int64_t rows;
+    int32_t K, x_type;             /* SD_BF16 or SD_F32 */
+    const void *x;                 /* [rows][K], rows x_stride elements apart */
+    int64_t x_stride;
+    void *q;                       /* out int8 [rows][K], rows q_stride bytes apart; bytes up to K rounded up to 16 are zero */
+    int64_t q_stride;
+    float *scale;                  /* out [rows] */
+} sd_quantize_rows_args;
+
+typedef struct {
+    int64_t rows;
+    int32_t N, K, swiglu;
+    int32_t x_type, y_type, bias_type;   /* SD_BF16, SD_F32, x also SD_I8 */
+    const void *x;                 /* [rows][K], rows x_stride elements apart */
+    int64_t x_stride;
+    const float *x_scale;          /* [rows], with SD_I8 */
+    const void *weight;            /* int8 [N][K], rows weight_stride bytes apart */
+    int64_t weight_stride;
+    const float *weight_scale;     /* [N] */
+    const void *bias;              /* [N] or NULL */
+    void *y;                       /* out [rows][N or N / 2], rows y_stride elements apart */
+    int64_t y_stride;
+    void *scratch;
+    size_t scratch_bytes;
+} sd_int8_linear_args;
+
+int sd_quantize_rows(const sd_quantize_rows_args *args, void *stream);
+size_t sd_int8_linear_scratch_bytes(const sd_int8_linear_args *args);
+int sd_int8_linear(const sd_int8_linear_args *args, void *stream);
+
+/*
+ * sd_sample_tokens  one token per row of logits, from one uniform number in [0, 1) per row.  Candidates in the
+ *                   order of their logits, equal ones by index, have weights exp((x - x_max) / temperature);
+ *                   top_k keeps the first k (0 or less: all), top_p those of them before which less than
+ *                   top_p of their weight lies (1 and above: all, 0 and below: the first), min_p those whose weight
+ *                   is at least min_p times the largest.  The token is the first index at which the running sum
+ *                   of the kept weights, in the order of the vocabulary, exceeds uniform times their sum.  A
+ *                   temperature of 0 (below 1e-30, or NaN) takes the first of the order.  Logits of -infinity
+ *                   and NaN are never drawn, those of +infinity share the draw; a row with nothing to draw gets
+ *                   empty_token.  Weights are 64-bit fixed point with 44 bits below the largest, so results do not
+ *                   depend on how the sums are split.  V <= 262144.
+ */
+typedef struct {
+    int64_t rows;
+    int32_t V, logits_type;        /* SD_BF16 or SD_F32 */
+    const void *logits;            /* [rows][V], rows stride elements apart */
+    int64_t stride;
+    const float *uniform;          /* [rows] */
+    /* one value per row, or NULL: the number below for all */
+    const float *temperature_row;
+    const int32_t *top_k_row;
+    const float *top_p_row;
+    const float *min_p_row;
+    double temperature, top_p, min_p;
+    int32_t top_k;
+    int64_t empty_token;
+    int64_t *tokens;               /* out [rows] */
+} sd_sample_tokens_args;
+
+int sd_sample_tokens(const sd_sample_tokens_args *args, void *stream);
+
 const char *sd_status_string(int status);
 int sd_version(void);
 /* Tokens per chunk of the chunked scan (a private tuning constant upstream). */

@@ -8,6 +8,7 @@ sm_100a CUDA kernels behind a C ABI (include/solvedelta_b200.h).
 """
 from ._lib import build, load
 from .config import SolveDeltaConfig
+from .int8_ops import int8_linear, int8_matmul, quantize_rows
 from .mixer_ops import conv4_silu, conv4_silu_segmented, kda_decay_gate, rms_norm_gated, rms_norm_gated_linear
 from .model import RMSNormGated, SolveDelta, SolveDeltaLayerState
 from .modeling import (GraphedDecoder, SolveDeltaBlock, SolveDeltaCache, SolveDeltaCacheAdapter, SolveDeltaForCausalLM,
@@ -15,6 +16,7 @@ from .modeling import (GraphedDecoder, SolveDeltaBlock, SolveDeltaCache, SolveDe
 from .training import (BF16ShadowWeights, BucketedGradientAverager, SolveDeltaGraphedTrainingStep,
                        allreduce_gradients, causal_lm_loss,
                        fixed_dense_linear_cross_entropy, fused_cross_entropy)
+from .sampling import sample_tokens
 from .packing import PackedSegments, build_packed_segments, pack_tokens, unpack_tokens
 from .ops import (
     SolveDeltaState,
@@ -71,4 +73,8 @@ __all__ = [
     "pack_tokens",
     "unpack_tokens",
     "solvedelta_zero_state",
+    "int8_linear",
+    "int8_matmul",
+    "quantize_rows",
+    "sample_tokens",
 ]

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import re
 import shutil
 import subprocess
 
@@ -22,21 +23,31 @@ LIB_PATH = os.path.join(_BUILD, "libsolvedelta_b200.so")
 DIAG_LIB_PATH = os.path.join(_BUILD, "libsolvedelta_b200_diag.so")
 # the host side of the entry points (checks, tensors, autograd node) as a Python extension over the C ABI
 HOST_PATH = os.path.join(_BUILD, "sd_host.so")
-HOST_SOURCES = [os.path.join(_SRC, n) for n in ("sd_host.cpp", "sd_host_glue.cpp")]
+HOST_SOURCES = [os.path.join(_SRC, n) for n in ("sd_host.cpp", "sd_host_glue.cpp", "sd_host_serving.cpp")]
 HEADER_PATH = os.path.join(_ROOT, "include", "solvedelta_b200.h")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--expt-extended-lambda", "-shared", "-Xcompiler", "-fPIC",
+    "--expt-extended-lambda", "-Xcompiler", "-fPIC",
 ]
 
 
-def _sources():
-    out = [HEADER_PATH]
-    for name in sorted(os.listdir(_SRC)):
-        if name.endswith((".cu", ".cuh", ".h")):
-            out.append(os.path.join(_SRC, name))
-    return out
+def _units():
+    return [os.path.join(_SRC, n) for n in sorted(os.listdir(_SRC)) if n.endswith(".cu")]
+
+
+def _sources(path: str):
+    """A source file and every header of this package that it includes, directly or not."""
+    seen, todo = [], [os.path.normpath(path)]
+    while todo:
+        path = todo.pop()
+        if path in seen or not os.path.exists(path):
+            continue
+        seen.append(path)
+        with open(path) as source:
+            todo += [os.path.normpath(os.path.join(os.path.dirname(path), name))
+                     for name in re.findall(r'^#include "([^"]+)"', source.read(), flags=re.M)]
+    return seen
 
 
 def _nvcc():
@@ -47,32 +58,38 @@ def _nvcc():
 
 
 def is_stale(path: str = LIB_PATH) -> bool:
+    """Whether ``path`` is missing or older than a source it is made from."""
     if not os.path.exists(path):
         return True
     built = os.path.getmtime(path)
-    return any(os.path.getmtime(s) > built for s in _sources())
+    return any(os.path.getmtime(s) > built for unit in _units() for s in _sources(unit))
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile csrc/*.cu into the in-tree shared libraries (sm_100a only): the product library and
-    its profiling twin."""
+    its profiling twin.  Every unit is an object of its own; only those whose sources changed are compiled again."""
     nvcc = _nvcc()
-    jobs = []
-    for path, extra in ((LIB_PATH, []), (DIAG_LIB_PATH, ["-DSD_DIAGNOSTICS"])):
+    jobs, links = [], []
+    for path, suffix, extra in ((LIB_PATH, ".o", []), (DIAG_LIB_PATH, ".diag.o", ["-DSD_DIAGNOSTICS"])):
         if not force and not is_stale(path):
             continue
         if nvcc is None:
             raise RuntimeError("nvcc not found: cannot build " + os.path.basename(path))
         os.makedirs(_BUILD, exist_ok=True)
-        units = [os.path.join(_SRC, n) for n in sorted(os.listdir(_SRC)) if n.endswith(".cu")]
-        cmd = [nvcc, *NVCC_FLAGS, *extra, "-o", path, *units]
-        if verbose:
-            cmd.insert(1, "-Xptxas")
-            cmd.insert(2, "-v")
-        jobs.append((cmd, subprocess.Popen(cmd)))   # the two builds run side by side
+        objects = []
+        for unit in _units():
+            objects.append(os.path.join(_BUILD, os.path.basename(unit)[:-3] + suffix))
+            if (not force and os.path.exists(objects[-1])
+                    and all(os.path.getmtime(s) <= os.path.getmtime(objects[-1]) for s in _sources(unit))):
+                continue
+            cmd = [nvcc, *NVCC_FLAGS, *extra, *(["-Xptxas", "-v"] if verbose else []), "-c", "-o", objects[-1], unit]
+            jobs.append((cmd, subprocess.Popen(cmd)))   # side by side
+        links.append([nvcc, *NVCC_FLAGS, "-shared", "-o", path, *objects])
     for cmd, proc in jobs:
         if proc.wait() != 0:
             raise subprocess.CalledProcessError(proc.returncode, cmd)
+    for cmd in links:
+        subprocess.check_call(cmd)
     _build_host(force)
     return LIB_PATH
 
@@ -257,6 +274,34 @@ class Conv4BackwardArgs(ctypes.Structure):
                 ("valid_mask", ctypes.c_void_p), ("reset_mask", ctypes.c_void_p)]
 
 
+# element types of the serving operators
+BF16, F32, I8 = 0, 1, 2
+
+
+class QuantizeRowsArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("K", ctypes.c_int32), ("x_type", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("q", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("scale", ctypes.c_void_p)]
+
+
+class Int8LinearArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("swiglu", ctypes.c_int32),
+                ("x_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("bias_type", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("x_scale", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("weight_stride", ctypes.c_int64), ("weight_scale", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64),
+                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t)]
+
+
+class SampleTokensArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("V", ctypes.c_int32), ("logits_type", ctypes.c_int32),
+                ("logits", ctypes.c_void_p), ("stride", ctypes.c_int64), ("uniform", ctypes.c_void_p),
+                ("temperature_row", ctypes.c_void_p), ("top_k_row", ctypes.c_void_p), ("top_p_row", ctypes.c_void_p),
+                ("min_p_row", ctypes.c_void_p), ("temperature", ctypes.c_double), ("top_p", ctypes.c_double),
+                ("min_p", ctypes.c_double), ("top_k", ctypes.c_int32), ("empty_token", ctypes.c_int64),
+                ("tokens", ctypes.c_void_p)]
+
+
 class KdaGateArgs(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("H", ctypes.c_int32), ("r", ctypes.c_int32),
                 ("raw", ctypes.c_void_p), ("log_rate", ctypes.c_void_p), ("bias", ctypes.c_void_p),
@@ -286,6 +331,7 @@ EXPORTS = (
     "sd_conv4_backward_scratch_bytes", "sd_conv4_silu_forward", "sd_conv4_silu_backward",
     "sd_kda_gate_backward_scratch_bytes", "sd_kda_gate_forward", "sd_kda_gate_backward",
     "sd_norm_gate_backward_scratch_bytes", "sd_norm_gate_forward", "sd_norm_gate_backward",
+    "sd_quantize_rows", "sd_int8_linear_scratch_bytes", "sd_int8_linear", "sd_sample_tokens",
 )
 
 _lib = None
@@ -389,9 +435,13 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
                          ("sd_gemv", GemvArgs),
                          ("sd_conv4_silu_forward", Conv4ForwardArgs), ("sd_conv4_silu_backward", Conv4BackwardArgs),
                          ("sd_kda_gate_forward", KdaGateArgs), ("sd_kda_gate_backward", KdaGateArgs),
-                         ("sd_norm_gate_forward", NormGateArgs), ("sd_norm_gate_backward", NormGateArgs)):
+                         ("sd_norm_gate_forward", NormGateArgs), ("sd_norm_gate_backward", NormGateArgs),
+                         ("sd_quantize_rows", QuantizeRowsArgs), ("sd_int8_linear", Int8LinearArgs),
+                         ("sd_sample_tokens", SampleTokensArgs)):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+    lib.sd_int8_linear_scratch_bytes.restype = ctypes.c_size_t
+    lib.sd_int8_linear_scratch_bytes.argtypes = [ctypes.POINTER(Int8LinearArgs)]
     lib.sd_device_fault.restype = ctypes.c_int
     lib.sd_device_fault.argtypes = []
     lib.sd_device_fault_clear.restype = ctypes.c_int

@@ -5,6 +5,7 @@
 
 #include "../../include/solvedelta_b200.h"
 #include "sd_diagnostics.h"
+#include "sd_internal.h"
 #include "sd_backward.cuh"
 #include "sd_backward_tc.cuh"
 #include "sd_common.cuh"
@@ -124,9 +125,6 @@ __device__ int g_scan_fault_word = 0;
 int* g_scan_fault_ptr[64] = {};
 // cuTensorMapEncodeTiled is a driver function; it is reached through the runtime so that the library
 // links against the runtime alone.
-typedef CUresult (*TensorMapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                      const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                      CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 TensorMapEncodeFn tensor_map_encoder() {
     static TensorMapEncodeFn encode = nullptr;
     if (encode == nullptr) {
@@ -634,6 +632,11 @@ int launch_decode(const DecodeParams& p, const MixerDecode& m, int streams, bool
 }
 
 }  // namespace
+
+namespace sd {
+TensorMapEncodeFn map_encoder() { return tensor_map_encoder(); }
+int* fault_word() { return configure_kernels() == cudaSuccess ? scan_fault_ptr() : nullptr; }
+}  // namespace sd
 
 extern "C" {
 

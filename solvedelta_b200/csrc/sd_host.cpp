@@ -208,4 +208,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("dense", &dense);
     m.def("residual_frame", &residual_frame);
     register_glue(m);
+    register_serving(m);
 }

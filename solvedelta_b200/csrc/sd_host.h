@@ -43,3 +43,4 @@ inline bool is_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() 
 inline sd_operand operand(const Tensor& t) { return sd_operand{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 
 void register_glue(py::module_& m);
+void register_serving(py::module_& m);

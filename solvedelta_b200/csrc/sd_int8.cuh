@@ -1,0 +1,541 @@
+// 8-bit projections: y[i][j] = sx[i] sw[j] sum_k q[i][k] W[j][k] (+ bias[j]), q and W in int8, the sum exact in int32.
+//
+// Quantised rows.  With a = max_k |x_k|:  scale = a / 127 (rounded to FP32),  q_k = 127 x_k / a rounded to the nearest whole
+// number, ties to even, of the exact quotient, so that the integers do not depend on the order of two roundings.  A row of
+// zeros has scale 0; a row that holds an infinity or a NaN gets zeros and the scale NaN, so all its products are NaN.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "sd_common.cuh"
+#include "sd_tc.cuh"
+
+namespace sd {
+
+// ---- quantised rows -----------------------------------------------------------------------------------------------
+struct QuantizeParams {
+    long long rows;
+    int K;
+    const void* x;
+    long long x_stride;   // elements
+    signed char* q;
+    long long q_stride;   // bytes
+    float* scale;
+};
+
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// What a row's largest magnitude (its bits) makes of the row.
+struct RowScale {
+    float scale, inverse;   // a / 127 and about 127 / a
+    double largest;
+    bool tiny, bad;         // tiny: the inverse may overflow, every entry is taken in 64 bits
+};
+__device__ __forceinline__ RowScale row_scale(unsigned largest_bits) {
+    RowScale r;
+    const float a = __uint_as_float(largest_bits);
+    r.bad = largest_bits >= 0x7f800000u;
+    r.scale = r.bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(a, 127.f);
+    r.tiny = a < 1e-30f;
+    r.inverse = r.tiny || r.bad ? 0.f : __fdiv_rn(127.f, a);
+    r.largest = a;
+    return r;
+}
+// 127 x / a rounded to nearest even.  x times the rounded inverse is at most 1.5 * 2^-23 of itself off, under 2^-15: only
+// where that leaves open which side of a half the quotient is on, 127 x is compared with half * a, both exact in 64 bits.
+__device__ __forceinline__ int quantize_value(float x, const RowScale& r) {
+    if (r.bad || x == 0.f) return 0;
+    const float t = x * r.inverse;
+    float n = rintf(t);
+    if (r.tiny || fabsf(fabsf(t - n) - 0.5f) < 3.1e-5f) {
+        if (r.tiny) return (int)rint(127.0 * (double)x / r.largest);
+        const double half = floor((double)t * 2.0 + 0.5) * 0.5, exact = 127.0 * (double)x, border = half * r.largest;
+        const double low = floor(half), up = low + 1.0;   // half is the odd multiple of 1/2 next to t
+        n = (float)(exact > border ? up : exact < border ? low : (fmod(low, 2.0) == 0.0 ? low : up));
+    }
+    return (int)n;
+}
+
+template <class T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Eight entries of a row from column c0 on, zeros past its end.
+template <class T, bool VEC>
+__device__ __forceinline__ void load_eight(const T* row, int c0, int K, float (&v)[8]) {
+    if (VEC && c0 + 8 <= K) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(row + c0);
+            const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = __bfloat1622float2(p[e]);
+                v[2 * e] = f.x;
+                v[2 * e + 1] = f.y;
+            }
+        } else {
+            const float4 a = *reinterpret_cast<const float4*>(row + c0), b = *reinterpret_cast<const float4*>(row + c0 + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c0 + e < K ? to_float(row[c0 + e]) : 0.f;
+}
+__device__ __forceinline__ unsigned quantize_four(const float* v, const RowScale& r) {
+    unsigned w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= (unsigned)(quantize_value(v[e], r) & 0xff) << (8 * e);
+    return w;
+}
+
+// One CTA per row: the row is read for its largest magnitude and again, then out of L1 or L2, for its entries.  q rows start
+// on 16-byte boundaries, q_stride covers K rounded up to 16, and the bytes past K are set to zero.
+constexpr int QUANT_THREADS = 256;
+template <class T, bool VEC>
+__global__ void __launch_bounds__(QUANT_THREADS) k_quantize_rows(QuantizeParams p) {
+    __shared__ unsigned s_max[QUANT_THREADS / 32];
+    chain_wait();
+    chain_release();
+    const T* row = reinterpret_cast<const T*>(p.x) + (long long)blockIdx.x * p.x_stride;
+    unsigned top = 0;
+    for (int c0 = threadIdx.x * 8; c0 < p.K; c0 += QUANT_THREADS * 8) {
+        float v[8];
+        load_eight<T, VEC>(row, c0, p.K, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = s_max[threadIdx.x & (QUANT_THREADS / 32 - 1)];
+    top = __reduce_max_sync(0xffffffffu, top);
+    const RowScale r = row_scale(top);
+    signed char* out = p.q + (long long)blockIdx.x * p.q_stride;
+    const int padded = (p.K + 15) / 16 * 16;
+    for (int c0 = threadIdx.x * 8; c0 < padded; c0 += QUANT_THREADS * 8) {
+        float v[8];
+        load_eight<T, VEC>(row, c0, p.K, v);
+        *reinterpret_cast<uint2*>(out + c0) = make_uint2(quantize_four(v, r), quantize_four(v + 4, r));
+    }
+    if (threadIdx.x == 0) p.scale[blockIdx.x] = r.scale;
+}
+
+// ---- the product --------------------------------------------------------------------------------------------------
+struct Int8Params {
+    int M, outs, K;            // rows, output columns (half of the weight's rows with SwiGLU), length of the sums
+    const float* x_scale;      // [M]
+    const float* w_scale;      // [N]
+    const void* bias;          // [N] or null
+    int bias_f32;
+    void* y;
+    long long y_stride;        // elements
+    int out_f32;
+    int tiles_m, tiles_n;
+};
+
+__device__ __forceinline__ float int8_bias(const Int8Params& p, int n) {
+    if (p.bias == nullptr) return 0.f;
+    return p.bias_f32 ? reinterpret_cast<const float*>(p.bias)[n]
+                      : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
+}
+// silu(gate) * value, both in FP32, rounded once by the store
+__device__ __forceinline__ float int8_gated(float gate, float value) { return gate * sigmoidf_(gate) * value; }
+
+// tcgen05.mma.kind::i8, int32 accumulators in tensor memory.  Per CTA: tiles of 128 rows by BN weight rows, both K-major
+// in shared memory as rows of 128 bytes with the 128-byte swizzle, loaded by TMA (which fills what lies outside with
+// zeros: ragged M, N and K need nothing else) into a ring of stages.  With SwiGLU the BN weight rows are BN / 2 gate rows
+// and the BN / 2 value rows that belong to them, so that one tile's accumulator holds both factors of its outputs.
+//
+// One CTA per SM stays for all its tiles.  One thread loads, one thread issues the products, eight warps empty the
+// accumulator, of which there are two, so that the products of a tile run under the epilogue of the one before.
+constexpr int I8_BM = 128, I8_BK = 128, I8_THREADS = 384, I8_EPILOGUE_WARP = 4, I8_EPILOGUE_THREADS = 256;
+constexpr int I8_GROUP = 8;   // row tiles that are walked together: their rows and the weight tiles stay in L2
+template <int BN>
+struct Int8Tile {
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr unsigned A_BYTES = I8_BM * I8_BK, B_BYTES = BN * I8_BK, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr unsigned TMEM_COLS = 2 * BN;
+    static constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + 1024;
+};
+
+__device__ __forceinline__ void tc_load_2d(unsigned smem, const CUtensorMap* map, int col, int row, unsigned bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem),
+        "l"(reinterpret_cast<unsigned long long>(map)), "r"(col), "r"(row), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void i8_mma(unsigned d_tmem, unsigned long long da, unsigned long long db, unsigned idesc,
+                                       unsigned accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// int32 accumulator (2 at bit 4), signed operands (1 at bits 7 and 10), both K-major, M = 128
+__host__ __device__ constexpr unsigned i8_idesc(int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(I8_BM >> 4) << 24);
+}
+
+// Eight (FP32) or eight (BF16) neighbouring outputs of a row.
+template <bool F32>
+__device__ __forceinline__ void int8_store8(const Int8Params& p, long long row, int col, const float (&v)[8], bool vec) {
+    if constexpr (F32) {
+        float* y = reinterpret_cast<float*>(p.y) + row * p.y_stride + col;
+        if (vec && col + 8 <= p.outs) {
+            *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < p.outs) y[e] = v[e];
+        }
+    } else {
+        __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + row * p.y_stride + col;
+        if (vec && col + 8 <= p.outs) {
+            uint4 w;
+            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+            *reinterpret_cast<uint4*>(y) = w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < p.outs) y[e] = __float2bfloat16_rn(v[e]);
+        }
+    }
+}
+
+template <int BN, bool GATED, bool F32>
+__global__ void __launch_bounds__(I8_THREADS, 1)
+k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, int* fault) {
+    using Tile = Int8Tile<BN>;
+    constexpr int S = Tile::STAGES, OUTS = GATED ? BN / 2 : BN;
+    extern __shared__ __align__(16) unsigned char i8_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * S + 4];   // full, empty, accumulator full, accumulator empty
+    __shared__ unsigned s_tmem;
+    __shared__ __align__(16) float s_scale[2][BN], s_bias[2][BN];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const unsigned ring = (tc_smem(i8_raw) + 1023u) & ~1023u;
+    const unsigned full0 = tc_smem(bars), empty0 = full0 + 8 * S, acc_full0 = empty0 + 8 * S, acc_empty0 = acc_full0 + 16;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2 * S + 2; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8 * i));
+        for (int i = 0; i < 2; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty0 + 8 * i), "r"(I8_EPILOGUE_THREADS));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&s_tmem)), "r"(Tile::TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    chain_wait();   // the set-up above runs under the kernel that writes the rows
+    chain_release();
+    const unsigned tbase = s_tmem;
+    const int tiles = p.tiles_m * p.tiles_n, blocks = (p.K + I8_BK - 1) / I8_BK;
+    // groups of I8_GROUP row tiles; inside one, the row tile changes first
+    const auto place = [&](int tile, int& m, int& n) {
+        const int per_group = I8_GROUP * p.tiles_n, g = tile / per_group, rest = tile - g * per_group;
+        const int height = min(I8_GROUP, p.tiles_m - g * I8_GROUP);
+        n = rest / height;
+        m = g * I8_GROUP + rest - n * height;
+    };
+
+    if (warp == 0) {   // ---- loads
+        if (lane == 0) {
+            int k = 0;   // stages filled so far
+            bool alive = true;
+            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+                int m, n;
+                place(tile, m, n);
+                for (int b = 0; b < blocks && alive; ++b, ++k) {
+                    const int s = k % S;
+                    if (k >= S) alive = tc_wait(empty0 + 8 * s, (k / S - 1) & 1);
+                    if (!alive) break;
+                    const unsigned bar = full0 + 8 * s, a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(Tile::STAGE_BYTES) : "memory");
+                    tc_load_2d(a, &x_map, b * I8_BK, m * I8_BM, bar);
+                    tc_load_2d(w, &w_map, b * I8_BK, n * OUTS, bar);
+                    if (GATED) tc_load_2d(w + Tile::B_BYTES / 2, &w_map, b * I8_BK, p.outs + n * OUTS, bar);
+                }
+            }
+            if (!alive) {
+                atomicExch(fault, 9);
+                for (int i = k > S ? k - S : 0; i < k; ++i) tc_wait(full0 + 8 * (i % S), (i / S) & 1);   // copies in flight
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {   // ---- products
+        if (lane == 0) {
+            int k = 0, t = 0;
+            bool alive = true;
+            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x, ++t) {
+                if (t >= 2) alive = tc_wait(acc_empty0 + 8 * (t & 1), (t / 2 - 1) & 1);
+                tc_fence_after();
+                const unsigned acc = tbase + (t & 1) * BN;
+                for (int b = 0; b < blocks && alive; ++b, ++k) {
+                    const int s = k % S;
+                    alive = tc_wait(full0 + 8 * s, (k / S) & 1);
+                    if (!alive) break;
+                    tc_fence_after();
+                    const unsigned a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
+#pragma unroll
+                    for (int j = 0; j < I8_BK / 32; ++j)
+                        i8_mma(acc, tc_desc(a + j * 32, 16, 1024) | (2ull << 61), tc_desc(w + j * 32, 16, 1024) | (2ull << 61),
+                               i8_idesc(BN), b > 0 || j > 0 ? 1u : 0u);
+                    tc_commit(empty0 + 8 * s);
+                }
+                if (alive) tc_commit(acc_full0 + 8 * (t & 1));
+            }
+            if (!alive) atomicExch(fault, 10);
+        }
+        __syncwarp();
+    } else if (warp >= I8_EPILOGUE_WARP) {   // ---- scales, bias, gate, store
+        const int quarter = warp & 3, half = (warp - I8_EPILOGUE_WARP) >> 2, etid = tid - I8_EPILOGUE_WARP * 32;
+        const int align = F32 ? 4 : 8;
+        const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.y_stride % align == 0;
+        int t = 0;
+        bool alive = true;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+            int m, n;
+            place(tile, m, n);
+            float *scale = s_scale[t & 1], *bias = s_bias[t & 1];
+            if (etid < BN) {
+                const int c = GATED ? etid % OUTS : etid, col = n * OUTS + c;
+                const int w = GATED && etid >= OUTS ? p.outs + col : col;
+                scale[etid] = col < p.outs ? p.w_scale[w] : 0.f;
+                bias[etid] = col < p.outs ? int8_bias(p, w) : 0.f;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(I8_EPILOGUE_THREADS) : "memory");
+            const int i = m * I8_BM + quarter * 32 + lane;
+            const float sx = i < p.M ? p.x_scale[i] : 0.f;
+            if (alive) alive = tc_wait(acc_full0 + 8 * (t & 1), (t / 2) & 1);
+            alive = __all_sync(0xffffffffu, alive);
+            if (!alive) {
+                if (lane == 0) atomicExch(fault, 11);
+                continue;   // nothing is read or stored any more
+            }
+            tc_fence_after();
+            const unsigned acc = tbase + (t & 1) * BN + ((unsigned)(quarter * 32) << 16);
+            constexpr int STEP = 16;
+#pragma unroll 1
+            for (int c0 = half * (OUTS / 2); c0 < (half + 1) * (OUTS / 2); c0 += STEP) {
+                float r[STEP], g[STEP];
+                tc_ld16(acc + c0, r);
+                if (GATED) tc_ld16(acc + OUTS + c0, g);
+                tc_wait_ld();
+#pragma unroll
+                for (int e8 = 0; e8 < STEP; e8 += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int c = c0 + e8 + e;
+                        v[e] = fmaf((float)__float_as_int(r[e8 + e]) * sx, scale[c], bias[c]);
+                        if (GATED)
+                            v[e] = int8_gated(v[e], fmaf((float)__float_as_int(g[e8 + e]) * sx, scale[OUTS + c], bias[OUTS + c]));
+                    }
+                    if (i < p.M && n * OUTS + c0 + e8 < p.outs) int8_store8<F32>(p, i, n * OUTS + c0 + e8, v, vec);
+                }
+            }
+            tc_fence_before();
+            tc_arrive(acc_empty0 + 8 * (t & 1));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(Tile::TMEM_COLS));
+}
+
+// ---- few rows: a cached token of a serving batch --------------------------------------------------------------------
+// Bound by the weight, read once, and behind that by the latency of one launch.  Two CTAs of eight warps per SM stay for
+// all their tiles of 8 CG weight rows (gate and value rows side by side with SwiGLU).  A warp takes one group of eight
+// weight rows and a slice of K; a lane keeps the 16-byte pieces of two steps in flight ahead of the products.  The products
+// run on mma.sync m16n8k32 with the rows of x as the M side: the contraction index is permuted so that a lane's 16-byte
+// piece of a weight row is its B fragment of two instructions, and the rows, in shared memory, are read with the same
+// permutation.  BF16 rows are quantised by every CTA on the way into shared memory.
+constexpr int I8_TOKEN_ROWS = 32;
+constexpr size_t I8_TOKEN_SMEM = 190 * 1024;
+constexpr int I8_TOKEN_BATCH = 4;
+// Row pitch in shared memory, 64 bytes off a multiple of 128: the eight 16-byte pieces a quarter-warp reads (two rows, four
+// consecutive pieces) fall into distinct banks.
+__host__ __device__ constexpr long long int8_pitch(int K) { return ((long long)K + 127) / 128 * 128 + 64; }
+
+struct Int8TokenParams {
+    Int8Params o;              // M, outs, K, scales, bias, y
+    const void* x;             // rows, x_stride elements apart
+    long long x_stride;
+    int vec;                   // rows of x start on 16-byte boundaries
+    const signed char* W;      // [N][w_stride], readable up to K rounded up to 16
+    long long w_stride;
+};
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A 16-byte piece of a weight row: read once by one CTA, and ahead of the wait for the kernel before.
+__device__ __forceinline__ uint4 load_piece(const signed char* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
+// The rows of x as int8 in shared memory, zeros past K; T: BF16 or FP32 rows are quantised, int8 rows are copied.
+template <class T, bool VEC>
+__device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char* s_q, float* s_scale, unsigned* s_top) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, M = p.o.M, K = p.o.K;
+    const int pitch = (int)int8_pitch(K);
+    if constexpr (sizeof(T) == 1) {
+        const int pieces = pitch / 16;
+        for (int idx = tid; idx < M * pieces; idx += 256) {
+            const int m = idx / pieces, c0 = (idx - m * pieces) * 16;
+            const signed char* row = reinterpret_cast<const signed char*>(p.x) + m * p.x_stride;
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (VEC && c0 + 16 <= K) {
+                w = *reinterpret_cast<const uint4*>(row + c0);
+            } else {
+                unsigned* u = reinterpret_cast<unsigned*>(&w);
+                for (int e = 0; e < 16; ++e)
+                    if (c0 + e < K) u[e / 4] |= (unsigned)(row[c0 + e] & 0xff) << (8 * (e % 4));
+            }
+            *reinterpret_cast<uint4*>(s_q + (long long)m * pitch + c0) = w;
+        }
+        if (tid < M) s_scale[tid] = p.o.x_scale[tid];
+    } else {
+        // units of 256 entries of a row, a warp each
+        const int segs = (pitch + 255) / 256;
+        if (tid < M) s_top[tid] = 0;
+        __syncthreads();
+        for (int u = warp; u < M * segs; u += 8) {
+            const int m = u / segs, c0 = (u - m * segs) * 256 + lane * 8;
+            float v[8];
+            load_eight<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K, v);
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) atomicMax(s_top + m, top);
+        }
+        __syncthreads();
+        for (int u = warp; u < M * segs; u += 8) {
+            const int m = u / segs, c0 = (u - m * segs) * 256 + lane * 8;
+            const RowScale r = row_scale(s_top[m]);
+            float v[8];
+            load_eight<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K, v);
+            if (c0 < pitch) *reinterpret_cast<uint2*>(s_q + (long long)m * pitch + c0) = make_uint2(quantize_four(v, r), quantize_four(v + 4, r));
+            if (c0 == 0) s_scale[m] = r.scale;
+        }
+    }
+}
+
+// RG: groups of eight rows; CG: groups of eight weight rows per CTA (2 with GATED)
+template <int RG, int CG, bool GATED, class T, bool VEC>
+__global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenParams p) {
+    static_assert(!GATED || CG == 2, "gate and value rows are the two groups");
+    constexpr int KS = 8 / CG, MT = (RG + 1) / 2, B = I8_TOKEN_BATCH;
+    extern __shared__ __align__(16) unsigned char i8_raw[];
+    signed char* s_q = reinterpret_cast<signed char*>(i8_raw);
+    __shared__ int s_red[2][8][RG * 8][9];
+    __shared__ float s_scale[RG * 8];
+    __shared__ unsigned s_top[RG * 8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int cg = warp % CG, ks = warp / CG, M = p.o.M, K = p.o.K, outs = p.o.outs;
+    constexpr int WIDTH = GATED ? 8 : 8 * CG;
+    const int tiles = (outs + WIDTH - 1) / WIDTH;
+    const int chunks = (K + 63) / 64, per = (chunks + KS - 1) / KS;
+    const int begin = min(ks * per, chunks), end = min(begin + per, chunks);
+    const int steps = (per + B - 1) / B;
+    const int mine = tiles > (int)blockIdx.x ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int total = mine * steps;
+    const int pitch = (int)int8_pitch(K);
+
+    const auto request = [&](int item, uint4 (&w)[B]) {
+        const int tile = blockIdx.x + item / steps * gridDim.x, base = begin + item % steps * B;
+        const int col = tile * WIDTH + (GATED ? g : cg * 8 + g);
+        const bool ok = item < total && col < outs;
+        const signed char* row = p.W + (long long)(GATED ? col + cg * outs : col) * p.w_stride + t * 16;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int c = base + i;
+            w[i] = ok && c < end && c * 64 + t * 16 < K ? load_piece(row + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    uint4 wa[B], wb[B];
+    request(0, wa);
+    request(1, wb);
+    chain_wait();
+    chain_release();
+    int8_rows<T, VEC>(p, s_q, s_scale, s_top);
+    __syncthreads();
+
+    int acc[MT][4];
+    const auto step = [&](int item, uint4 (&w)[B]) {
+        const int st = item % steps, base = begin + st * B;
+        if (st == 0) {
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[a][e] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            if (base + i < end) {   // warp-uniform
+                const signed char* sx = s_q + (base + i) * 64 + t * 16;
+#pragma unroll
+                for (int a = 0; a < MT; ++a) {
+                    const int r0 = a * 16 + g, r1 = r0 + 8;
+                    const uint4 lo = r0 < M ? *reinterpret_cast<const uint4*>(sx + r0 * pitch) : make_uint4(0u, 0u, 0u, 0u);
+                    const uint4 hi = 2 * a + 1 < RG && r1 < M ? *reinterpret_cast<const uint4*>(sx + r1 * pitch) : make_uint4(0u, 0u, 0u, 0u);
+                    mma_s8(acc[a], lo.x, hi.x, lo.y, hi.y, w[i].x, w[i].y);
+                    mma_s8(acc[a], lo.z, hi.z, lo.w, hi.w, w[i].z, w[i].w);
+                }
+            }
+        }
+        request(item + 2, w);
+        if (st != steps - 1) return;
+        // last step of a tile: the K slices are added up through shared memory (two buffers in turn, so one barrier)
+        const int tile_no = item / steps, buf = tile_no & 1;
+#pragma unroll
+        for (int a = 0; a < MT; ++a) {
+            s_red[buf][warp][a * 16 + g][2 * t] = acc[a][0];
+            s_red[buf][warp][a * 16 + g][2 * t + 1] = acc[a][1];
+            if (2 * a + 1 < RG) {
+                s_red[buf][warp][a * 16 + 8 + g][2 * t] = acc[a][2];
+                s_red[buf][warp][a * 16 + 8 + g][2 * t + 1] = acc[a][3];
+            }
+        }
+        __syncthreads();
+        const int n0 = (blockIdx.x + tile_no * gridDim.x) * WIDTH;
+        for (int idx = tid; idx < M * WIDTH; idx += 256) {
+            const int m = idx / WIDTH, c = idx - m * WIDTH, n = n0 + c;
+            if (n >= outs) continue;
+            const auto value = [&](int group, int w_row) {
+                int v = 0;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) v += s_red[buf][k * CG + group][m][c & 7];
+                return fmaf((float)v * s_scale[m], p.o.w_scale[w_row], int8_bias(p.o, w_row));
+            };
+            float out = value(GATED ? 0 : c >> 3, n);
+            if (GATED) out = int8_gated(out, value(1, n + outs));
+            if (p.o.out_f32) reinterpret_cast<float*>(p.o.y)[m * p.o.y_stride + n] = out;
+            else reinterpret_cast<__nv_bfloat16*>(p.o.y)[m * p.o.y_stride + n] = __float2bfloat16_rn(out);
+        }
+    };
+    for (int item = 0; item < total; item += 2) {
+        step(item, wa);
+        if (item + 1 < total) step(item + 1, wb);
+    }
+}
+
+}  // namespace sd

@@ -1,0 +1,252 @@
+// C ABI of the serving operators: 8-bit projections and token sampling (declarations: include/solvedelta_b200.h).
+#include "../../include/solvedelta_b200.h"
+#include "sd_int8.cuh"
+#include "sd_internal.h"
+#include "sd_sampling.cuh"
+
+namespace {
+
+using namespace sd;
+
+bool aligned(const void* p, size_t n = 16) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int status_of(cudaError_t e) {
+    const cudaError_t last = cudaGetLastError();
+    return e == cudaSuccess && last == cudaSuccess ? SD_OK : SD_ERR_LAUNCH_FAILED;
+}
+
+// Opt-in to dynamic shared memory above the default, once per device and kernel, always to the same size.
+template <auto KERNEL>
+cudaError_t allow_smem(size_t most) {
+    static bool done[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+    if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most)) != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) done[dev] = true;
+    return cudaSuccess;
+}
+// `chained`: the kernel may start while the one before it in the stream still runs (it waits for it itself).
+template <auto KERNEL, class... Args>
+int launch(unsigned grid, unsigned threads, size_t smem, size_t most_smem, int cluster, bool chained, cudaStream_t stream, const Args&... args) {
+    if (most_smem > 0) {
+        const cudaError_t e = allow_smem<KERNEL>(most_smem);
+        if (e != cudaSuccess) return SD_ERR_NO_DEVICE;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2] = {};
+    int n = 0;
+    if (chained) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    return status_of(cudaLaunchKernelEx(&cfg, KERNEL, args...));
+}
+
+constexpr int MAX_K = 131072;   // 127 * 127 * K stays below 2^31
+int padded(int K) { return (K + 15) / 16 * 16; }
+
+// ---- quantised rows ----
+int quantize(const sd_quantize_rows_args* a, bool chained, cudaStream_t stream) {
+    QuantizeParams p{};
+    p.rows = a->rows; p.K = a->K;
+    p.x = a->x; p.x_stride = a->x_stride;
+    p.q = reinterpret_cast<signed char*>(a->q); p.q_stride = a->q_stride;
+    p.scale = a->scale;
+    const bool f32 = a->x_type == SD_F32;
+    const bool vec = aligned(a->x) && a->x_stride % (f32 ? 4 : 8) == 0;
+    const unsigned rows = (unsigned)a->rows;
+    if (f32) return vec ? launch<k_quantize_rows<float, true>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p)
+                        : launch<k_quantize_rows<float, false>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p);
+    return vec ? launch<k_quantize_rows<__nv_bfloat16, true>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p)
+               : launch<k_quantize_rows<__nv_bfloat16, false>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p);
+}
+
+// ---- products ----
+// Tensor map of int8 rows [rows][K]: boxes of `box_rows` rows by 128 bytes, 128-byte swizzle.
+bool int8_map(CUtensorMap* map, const void* base, long long rows, int K, long long stride, int box_rows) {
+    const TensorMapEncodeFn encode = map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)I8_BK, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, bool GATED, bool F32>
+int launch_matmul(Int8Params p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
+    constexpr int OUTS = GATED ? BN / 2 : BN;
+    CUtensorMap x_map, w_map;
+    int* fault = fault_word();
+    if (fault == nullptr) return SD_ERR_NO_DEVICE;
+    if (!int8_map(&x_map, q, p.M, p.K, q_stride, I8_BM) || !int8_map(&w_map, a->weight, a->N, p.K, a->weight_stride, OUTS))
+        return SD_ERR_LAUNCH_FAILED;
+    p.tiles_m = (p.M + I8_BM - 1) / I8_BM;
+    p.tiles_n = (p.outs + OUTS - 1) / OUTS;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    if (tiles > 0x7fffffffLL - 148) return SD_ERR_UNSUPPORTED_SHAPE;
+    return launch<k_int8_matmul<BN, GATED, F32>>((unsigned)(tiles < 148 ? tiles : 148), I8_THREADS, Int8Tile<BN>::SMEM,
+                                                 Int8Tile<BN>::SMEM, 1, chained, stream, p, x_map, w_map, fault);
+}
+template <bool GATED, bool F32>
+int matmul_tile(const Int8Params& p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
+    const auto tiles = [&](int bn) {
+        const int outs = GATED ? bn / 2 : bn;
+        return (long long)((p.M + I8_BM - 1) / I8_BM) * ((p.outs + outs - 1) / outs);
+    };
+    // the widest tile that still gives every SM one
+    if (tiles(256) >= 148) return launch_matmul<256, GATED, F32>(p, a, q, q_stride, chained, stream);
+    if (tiles(128) >= 148) return launch_matmul<128, GATED, F32>(p, a, q, q_stride, chained, stream);
+    return launch_matmul<64, GATED, F32>(p, a, q, q_stride, chained, stream);
+}
+int matmul(const Int8Params& p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
+    if (a->swiglu) return p.out_f32 ? matmul_tile<true, true>(p, a, q, q_stride, chained, stream)
+                                    : matmul_tile<true, false>(p, a, q, q_stride, chained, stream);
+    return p.out_f32 ? matmul_tile<false, true>(p, a, q, q_stride, chained, stream)
+                     : matmul_tile<false, false>(p, a, q, q_stride, chained, stream);
+}
+
+size_t token_smem(int M, int K) { return (size_t)(M * int8_pitch(K)); }
+template <int RG, int CG, bool GATED, class T, bool VEC>
+int launch_token(const Int8TokenParams& p, bool chained, cudaStream_t stream) {
+    constexpr int WIDTH = GATED ? 8 : 8 * CG;
+    const int tiles = (p.o.outs + WIDTH - 1) / WIDTH;
+    const size_t smem = token_smem(p.o.M, p.o.K);
+    const int resident = 148 * (RG <= 2 && smem <= 96 * 1024 ? 2 : 1);
+    return launch<k_int8_token<RG, CG, GATED, T, VEC>>((unsigned)(tiles < resident ? tiles : resident), 256, smem, I8_TOKEN_SMEM, 1,
+                                                       chained, stream, p);
+}
+template <int RG, class T, bool VEC>
+int token_width(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t stream) {
+    if (gated) return launch_token<RG, 2, true, T, VEC>(p, chained, stream);
+    // 16 columns a tile while that gives every SM one, else 8
+    return p.o.outs >= 16 * 148 ? launch_token<RG, 2, false, T, VEC>(p, chained, stream)
+                                : launch_token<RG, 1, false, T, VEC>(p, chained, stream);
+}
+template <class T, bool VEC>
+int token_rows(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t stream) {
+    if (p.o.M <= 8) return token_width<1, T, VEC>(p, gated, chained, stream);
+    if (p.o.M <= 16) return token_width<2, T, VEC>(p, gated, chained, stream);
+    return token_width<4, T, VEC>(p, gated, chained, stream);
+}
+bool token_takes(const sd_int8_linear_args* a) { return a->rows <= I8_TOKEN_ROWS && token_smem((int)a->rows, a->K) <= I8_TOKEN_SMEM; }
+// Few entries: every CTA quantises the rows for itself, which saves a launch; past that its reading costs more.
+constexpr long long TOKEN_FUSED_ENTRIES = 16384;
+bool token_fuses(const sd_int8_linear_args* a) {
+    return token_takes(a) && a->x_type == SD_BF16 && aligned(a->x) && a->x_stride % 8 == 0 && a->rows * a->K <= TOKEN_FUSED_ENTRIES;
+}
+
+size_t q_bytes(const sd_int8_linear_args* a) { return ((size_t)a->rows * padded(a->K) + 255) / 256 * 256; }
+
+// ---- sampling ----
+constexpr size_t SAMPLE_SLICE_BYTES = 96 * 1024;   // of a CTA, where eight CTAs a row are not too few
+constexpr size_t SAMPLE_SMEM = 132 * 1024;         // a slice of the largest vocabulary in FP32 over eight CTAs, and its alignment
+static_assert((SAMPLE_MAX_VOCAB / 8 + 8) * 4 <= SAMPLE_SMEM, "the largest slice");
+template <class T, int C>
+int launch_sample(SampleParams p, long long rows, cudaStream_t stream) {
+    constexpr int VE = 16 / sizeof(T);
+    // rows may start up to VE - 1 elements behind a 16-byte boundary
+    p.slice = ((p.V + VE - 1 + C - 1) / C + VE - 1) / VE * VE;
+    return launch<k_sample<T, C>>((unsigned)(rows * C), SAMPLE_THREADS, (size_t)p.slice * sizeof(T), SAMPLE_SMEM, C, false, stream, p);
+}
+template <class T>
+int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
+    // as many CTAs a row as keep the SMs busy, with slices of 2048 entries at least and 96 KB at most
+    const auto fits = [&](int c) { return (size_t)p.V * sizeof(T) <= c * SAMPLE_SLICE_BYTES; };
+    const auto worth = [&](int c) { return rows * c <= 148 && p.V >= c * 2048; };
+    if (worth(8) || !fits(4)) return launch_sample<T, 8>(p, rows, stream);
+    if (worth(4) || !fits(2)) return launch_sample<T, 4>(p, rows, stream);
+    if (worth(2) || !fits(1)) return launch_sample<T, 2>(p, rows, stream);
+    return launch_sample<T, 1>(p, rows, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sd_quantize_rows(const sd_quantize_rows_args* a, void* stream_) {
+    if (!a || a->rows <= 0 || a->K <= 0 || !a->x || !a->q || !a->scale || (a->x_type != SD_BF16 && a->x_type != SD_F32))
+        return SD_ERR_INVALID_ARGUMENT;
+    if (a->q_stride < padded(a->K) || a->q_stride % 16 != 0 || !aligned(a->q)) return SD_ERR_INVALID_ARGUMENT;
+    if (a->rows > 0x7fffffffLL || a->K > MAX_K) return SD_ERR_UNSUPPORTED_SHAPE;
+    return quantize(a, false, reinterpret_cast<cudaStream_t>(stream_));
+}
+
+size_t sd_int8_linear_scratch_bytes(const sd_int8_linear_args* a) {
+    if (!a || a->rows <= 0 || a->K <= 0 || a->x_type == SD_I8 || token_fuses(a)) return 0;
+    return q_bytes(a) + (size_t)a->rows * 4;
+}
+
+int sd_int8_linear(const sd_int8_linear_args* a, void* stream_) {
+    if (!a || a->rows <= 0 || a->N <= 0 || a->K <= 0 || !a->x || !a->weight || !a->weight_scale || !a->y ||
+        (a->swiglu && a->N % 2 != 0) || (a->y_type != SD_BF16 && a->y_type != SD_F32) || a->x_type < SD_BF16 || a->x_type > SD_I8 ||
+        (a->x_type == SD_I8 && !a->x_scale) || (a->bias && a->bias_type != SD_BF16 && a->bias_type != SD_F32))
+        return SD_ERR_INVALID_ARGUMENT;
+    if (!aligned(a->weight) || a->weight_stride % 16 != 0 || a->weight_stride < padded(a->K) ||
+        (a->x_type == SD_I8 && (!aligned(a->x) || a->x_stride % 16 != 0 || (a->rows > 1 && a->x_stride < padded(a->K)))))
+        return SD_ERR_INVALID_ARGUMENT;
+    if (a->K > MAX_K || a->rows > 0x7fffff00LL) return SD_ERR_UNSUPPORTED_SHAPE;
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    Int8Params p{};
+    p.M = (int)a->rows; p.outs = a->swiglu ? a->N / 2 : a->N; p.K = a->K;
+    p.x_scale = a->x_scale; p.w_scale = a->weight_scale;
+    p.bias = a->bias; p.bias_f32 = a->bias_type == SD_F32;
+    p.y = a->y; p.y_stride = a->y_stride; p.out_f32 = a->y_type == SD_F32;
+    const bool token = token_takes(a);
+    Int8TokenParams t{};
+    t.W = reinterpret_cast<const signed char*>(a->weight); t.w_stride = a->weight_stride;
+    if (token_fuses(a)) {
+        t.o = p; t.x = a->x; t.x_stride = a->x_stride;
+        return token_rows<__nv_bfloat16, true>(t, a->swiglu != 0, false, stream);
+    }
+    const void* q = a->x;
+    long long q_stride = a->x_stride;
+    const bool quantized = a->x_type == SD_I8;
+    if (!quantized) {
+        if (!a->scratch || !aligned(a->scratch) || a->scratch_bytes < sd_int8_linear_scratch_bytes(a)) return SD_ERR_BUFFER_TOO_SMALL;
+        sd_quantize_rows_args r{};
+        r.rows = a->rows; r.K = a->K; r.x_type = a->x_type; r.x = a->x; r.x_stride = a->x_stride;
+        r.q = a->scratch; r.q_stride = padded(a->K);
+        r.scale = reinterpret_cast<float*>(reinterpret_cast<char*>(a->scratch) + q_bytes(a));
+        const int e = quantize(&r, false, stream);
+        if (e != SD_OK) return e;
+        q = r.q; q_stride = r.q_stride; p.x_scale = r.scale;
+    }
+    if (token) {
+        t.o = p; t.x = q; t.x_stride = q_stride;
+        return token_rows<signed char, true>(t, a->swiglu != 0, !quantized, stream);
+    }
+    return matmul(p, a, q, q_stride, !quantized, stream);
+}
+
+int sd_sample_tokens(const sd_sample_tokens_args* a, void* stream_) {
+    if (!a || a->rows <= 0 || a->V <= 0 || !a->logits || !a->uniform || !a->tokens ||
+        (a->logits_type != SD_BF16 && a->logits_type != SD_F32) || !aligned(a->logits, a->logits_type == SD_F32 ? 4 : 2))
+        return SD_ERR_INVALID_ARGUMENT;
+    if (a->V > SAMPLE_MAX_VOCAB || a->rows > (0x7fffffffLL >> 3)) return SD_ERR_UNSUPPORTED_SHAPE;
+    SampleParams p{};
+    p.V = a->V;
+    p.logits = a->logits; p.stride = a->stride; p.uniform = a->uniform;
+    p.temperature_row = a->temperature_row; p.top_k_row = a->top_k_row; p.top_p_row = a->top_p_row; p.min_p_row = a->min_p_row;
+    p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
+    p.empty_token = a->empty_token;
+    p.tokens = reinterpret_cast<long long*>(a->tokens);
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    return a->logits_type == SD_F32 ? sample<float>(p, a->rows, stream) : sample<__nv_bfloat16>(p, a->rows, stream);
+}
+
+}  // extern "C"
