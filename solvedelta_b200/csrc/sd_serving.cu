@@ -167,7 +167,7 @@ template <class T>
 int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
     // as many CTAs a row as keep the SMs busy, with slices of 2048 entries at least and 96 KB at most
     const auto fits = [&](int c) { return (size_t)p.V * sizeof(T) <= c * SAMPLE_SLICE_BYTES; };
-    const auto worth = [&](int c) { return rows * c <= 148 && p.V >= c * 2048; };
+    const auto worth = [&](int c) { return rows * c <= 2 * 148 && p.V >= c * 2048; };
     if (worth(8) || !fits(4)) return launch_sample<T, 8>(p, rows, stream);
     if (worth(4) || !fits(2)) return launch_sample<T, 4>(p, rows, stream);
     if (worth(2) || !fits(1)) return launch_sample<T, 2>(p, rows, stream);

@@ -22,7 +22,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: U
     ``uniform`` times their sum.  ``temperature`` 0 takes the first of the order.  Each setting is a number or a tensor
     ``[B]`` on the device of the logits, one value for each row (numbers out of range are refused; in a tensor a
     temperature that is not above 1e-30 and a ``top_p`` that is not above 0 take the first of the order, a ``top_k``
-    below 1, a ``top_p`` above 1 and a ``min_p`` below 0 keep all, a ``min_p`` above 1 counts as 1).
+    below 1, a ``top_p`` above 1 and a ``min_p`` below 0 keep all, a ``min_p`` above 1 counts as 1).  A
+    temperature above 1e30 counts as 1e30.
 
     Logits of -inf and NaN are never drawn; those of +inf share the draw.  A row that has nothing to draw gets
     ``empty_token``.  The weights are exact to 2^-45 of the largest and their sums are exact, so a row's token does not
