@@ -11,14 +11,16 @@
 // exact whatever their order, so results depend neither on the split of a row nor on the order of atomics, and a drawn
 // index differs from that of real numbers only where u is within about 1e-11 of a border.  A weight under 2^-45 is zero.
 //
-// A row is kept in shared memory by a cluster of C CTAs, contiguous slices of the vocabulary, a contiguous range a warp.
-// A rule first takes a histogram of the row over 1024 equal steps of (x_max - x) / T, of counts (top-k) or of weights to 16
+// A row is split over a cluster of C CTAs, contiguous slices of the vocabulary, and over their warps.  Short slices are kept
+// in shared memory; of long ones (many rows of a large vocabulary) every pass reads the row again, out of L2, through a ring
+// of asynchronous copies.
+// A rule first takes a histogram of the row over steps of a 16th of a binade of the weight, of counts (top-k) or of weights to 16
 // bits (top-p), which says in which step its border lies at most.  What is in front of that is all that can be drawn:
 // * up to 512 candidates go to the first CTA, one a thread, which sorts them, sums them up and draws;
-// * more are moved together by their warps, in place.  The exact border comes from a histogram over them and from further
-//   ones, over equal steps of the logit's bits, until one value is left; sums and draw go over what was moved.
+// * more are moved together by their warps.  The exact border comes from the entries of its step, gathered, or, where those
+//   are more than 512, from further histograms over equal steps of the logit's bits, until one value is left; sums and draw
+//   go over what was moved.
 #pragma once
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -41,6 +43,7 @@ struct SampleParams {
     long long empty_token;
     long long* tokens;
     int slice;                 // elements of a CTA's slice, a multiple of 16 bytes
+    int list;                  // rows that are read again: entries a warp can move together
 };
 
 constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32, SAMPLE_BINS = 2 * SAMPLE_THREADS;
@@ -49,8 +52,15 @@ static_assert(SAMPLE_GROUPS == 32 && SAMPLE_GROUPS == 2 * SAMPLE_WARPS, "a lane 
 constexpr int SAMPLE_WEIGHT_BITS = 44;
 constexpr int SAMPLE_RANGE = 45;          // binades under the largest weight that are not rounded to zero
 constexpr int SAMPLE_TABLE = 128;         // steps of a binade in the exponential's table
+constexpr int SAMPLE_BIN_BITS = 3;        // eight of them are a bin
+constexpr float SAMPLE_FAR = 63.9f;       // binades, where the last bin ends
+static_assert(int(SAMPLE_FAR * SAMPLE_TABLE) >> SAMPLE_BIN_BITS < SAMPLE_BINS, "bins");
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
+constexpr int SAMPLE_RING = 4;            // vectors a lane has in flight, where the row is read again
+constexpr size_t SAMPLE_RING_BYTES = size_t(SAMPLE_THREADS) * 16 * SAMPLE_RING;
 typedef unsigned long long u64;
+// the kernel's parts share its variables by reference: one that is not inlined would keep them in local memory
+#define SAMPLE_INLINE __attribute__((always_inline))
 
 // Order-preserving bits of a float, and back.
 __device__ __forceinline__ unsigned order_bits(float x) {
@@ -62,7 +72,7 @@ __device__ __forceinline__ float from_order_bits(unsigned k) {
 }
 
 struct SampleShared {
-    double power[SAMPLE_TABLE];   // 2^(j / SAMPLE_TABLE)
+    double power[SAMPLE_TABLE];   // 2^(-j / SAMPLE_TABLE)
     unsigned count[SAMPLE_BINS];
     u64 mass[SAMPLE_BINS];
     u64 group_mass[SAMPLE_GROUPS];
@@ -75,46 +85,74 @@ struct SampleShared {
     unsigned total_eq;
     unsigned kept;                // of the slice: entries in front of the border (written once)
     unsigned low, high;           // of the slice: smallest and largest bits in a step
+    unsigned in_step;             // of the slice: entries of the border's step
     int bin;
     unsigned bin_count;
     u64 before;
+    float edge;
+    unsigned ties;
 };
 
-// 2^(44 - t) to the nearest whole number, t in steps of 1 / 128 binade, 0 <= t < 45 * 128: with n the whole number next to
-// -t, 2^(n / 128) from a table and an exponent, and 2^(r / 128) for the rest |r| <= 1/2 from the exponential's series, cut
-// behind the fourth power (the term left out is below 2^-49).  Table-driven exponential: P. T. P. Tang, ACM TOMS 15 (1989).
-__device__ __forceinline__ u64 fixed_power(double t, const double* table) {
-    constexpr double ROUND = 6755399441055744.0;   // 1.5 * 2^52: a sum with it is rounded to a whole number
-    constexpr double L = 0.693147180559945309417 / SAMPLE_TABLE;
-    const double shifted = ROUND - t;
-    const double r = (ROUND - shifted) - t;
-    const int n = __double2loint(shifted);
+// 2^(44 - (n + r) / 128) to the nearest whole number, 0 <= n < 45 * 128 and |r| little over 1/2: 2^(-n / 128) from a table and
+// an exponent, 2^(-r / 128) from the exponential's series, cut behind the fourth power (the term left out is below 2^-49).
+// Table-driven exponential: P. T. P. Tang, ACM TOMS 15 (1989).
+__device__ __forceinline__ u64 fixed_power(int n, double r, const double* table) {
+    constexpr double L = -0.693147180559945309417 / SAMPLE_TABLE;
     double e = fma(r, L * L * L * L / 24, L * L * L / 6);
     e = fma(r, e, L * L / 2);
     e = fma(r, e, L);
     e = fma(r, e, 1.0);
     const double p = table[n & (SAMPLE_TABLE - 1)];
-    const double scaled = __hiloint2double(__double2hiint(p) + (((n >> 7) + SAMPLE_WEIGHT_BITS) << 20), __double2loint(p));
+    const double scaled = __hiloint2double(__double2hiint(p) + ((SAMPLE_WEIGHT_BITS - (n >> 7)) << 20), __double2loint(p));
     return (u64)__double_as_longlong(fma(e, scaled, 0x1p52)) - (u64)__double_as_longlong(0x1p52);
 }
 static_assert(SAMPLE_TABLE == 128, "fixed_power shifts by seven bits");
 
-template <class T, int C>
+// Shared memory of CTA `r` of the cluster, at the place of `p` in this one.
+__device__ __forceinline__ unsigned cluster_address(const void* p, int r) {
+    unsigned a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc_smem(p)), "r"(r));
+    return a;
+}
+__device__ __forceinline__ unsigned cluster_load(const unsigned* p, int r) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_address(p, r)) : "memory");
+    return v;
+}
+__device__ __forceinline__ u64 cluster_load(const u64* p, int r) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_address(p, r)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float cluster_load(const float* p, int r) {
+    return __uint_as_float(cluster_load(reinterpret_cast<const unsigned*>(p), r));
+}
+__device__ __forceinline__ void cluster_store(unsigned* p, int r, unsigned v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_address(p, r)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_store(u64* p, int r, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(p, r)), "l"(v) : "memory");
+}
+
+template <class T, int C, bool STAGED>
 __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
-    namespace cg = cooperative_groups;
     constexpr int VE = 16 / sizeof(T);
     extern __shared__ __align__(16) unsigned char smp_raw[];
-    T* s_x = reinterpret_cast<T*>(smp_raw);
+    T* s_x = reinterpret_cast<T*>(smp_raw);   // STAGED: the slice
     __shared__ SampleShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / C, rank = blockIdx.x % C;
-    const auto everywhere = [&]() {   // a barrier of all CTAs of the row
+    const auto everywhere = [&]() SAMPLE_INLINE {   // a barrier of all CTAs of the row
         if constexpr (C == 1) __syncthreads();
-        else cg::this_cluster().sync();
+        else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     };
-    const auto of_rank = [&](auto* ptr, int r) {
-        if constexpr (C == 1) return ptr;
-        else return cg::this_cluster().map_shared_rank(ptr, r);
+    const auto read = [&](const auto* ptr, int r) SAMPLE_INLINE {
+        if constexpr (C == 1) return *ptr;
+        else return cluster_load(ptr, r);
+    };
+    const auto write = [&](auto* ptr, int r, auto v) SAMPLE_INLINE {
+        if constexpr (C == 1) *ptr = v;
+        else cluster_store(ptr, r, v);
     };
     // The row starts `shift` elements behind a 16-byte boundary; positions count from that boundary, so that the vectors of
     // a slice are aligned in both memories.  Vectors that reach outside the row are read element by element.
@@ -122,9 +160,15 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     const int first = rank * p.slice, vectors = max(0, min(p.slice, p.V + shift - first) + VE - 1) / VE;
     const int per_warp = (vectors + SAMPLE_WARPS - 1) / SAMPLE_WARPS, v0 = min(vectors, warp * per_warp), v1 = min(vectors, v0 + per_warp);
-    T* const mine = s_x + v0 * VE;        // the warp's range
-    int held = (v1 - v0) * VE;            // and how many entries it still holds
-    const auto load = [&](int v, T (&e)[VE]) {
+    // what the warp holds in shared memory: its range, later what it moved together (`held` entries); rows that are read again
+    // have a ring of copies first, and a list with the entries' places in the warp's range behind it
+    T* const mine = STAGED ? s_x + v0 * VE : reinterpret_cast<T*>(smp_raw + SAMPLE_RING_BYTES) + warp * p.list;
+    unsigned short* const places =
+        reinterpret_cast<unsigned short*>(smp_raw + SAMPLE_RING_BYTES + sizeof(T) * SAMPLE_WARPS * p.list) + warp * p.list;
+    unsigned char* const ring = smp_raw + warp * (512 * SAMPLE_RING) + lane * 16;
+    bool here = STAGED;
+    int held = (v1 - v0) * VE;
+    const auto load = [&](int v, T (&e)[VE]) SAMPLE_INLINE {
         const int at = first + v * VE - shift;   // index of the vector's first element in the row
         if (at >= 0 && at + VE <= p.V) {
             *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x + at);
@@ -134,23 +178,82 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         }
     };
 
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int v = v0 + lane; v < v1; v += 32) {
-        alignas(16) T e[VE];
-        load(v, e);
+    bool infinite = false;   // there are infinite logits: they count as zeros, everything else as -infinity
+    const auto clean = [&](T (&e)[VE]) SAMPLE_INLINE {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
             const float f = to_float(e[j]);
             if (f != f) e[j] = T(-INFINITY);   // a NaN is never drawn
-            else top = fmaxf(top, f);
+            else if (infinite) e[j] = f == INFINITY ? T(0.f) : T(-INFINITY);
         }
-        *reinterpret_cast<uint4*>(s_x + v * VE) = *reinterpret_cast<const uint4*>(e);
+    };
+    // The vectors of the warp's range, 32 at a time: f(v, entries), all lanes together (v past the range: -infinity).
+    const auto scan_range = [&](auto&& f) SAMPLE_INLINE {
+        alignas(16) T e[VE];
+        if constexpr (STAGED) {
+            for (int base = v0; base < v1; base += 32) {
+                const int v = base + lane;
+                if (v < v1) {
+                    *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(s_x + v * VE);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) e[j] = T(-INFINITY);
+                }
+                f(v, e);
+            }
+        } else {
+            const auto inside = [&](int v) SAMPLE_INLINE { return first + v * VE - shift >= 0 && first + v * VE - shift + VE <= p.V; };
+            const auto request = [&](int base) SAMPLE_INLINE {
+                const int v = base + lane;
+                if (v < v1 && inside(v)) {
+                    const unsigned to = tc_smem(ring + (base / 32 % SAMPLE_RING) * 512);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(x + first + v * VE - shift) : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            // positions in the ring go by base / 32, whatever v0 is
+#pragma unroll
+            for (int k = 0; k < SAMPLE_RING - 1; ++k) request(v0 + 32 * k);
+            for (int base = v0; base < v1; base += 32) {
+                request(base + 32 * (SAMPLE_RING - 1));
+                asm volatile("cp.async.wait_group %0;" ::"n"(SAMPLE_RING - 1) : "memory");
+                const int v = base + lane;
+                if (v < v1 && inside(v)) {
+                    *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(ring + (base / 32 % SAMPLE_RING) * 512);
+                } else if (v < v1) {
+                    load(v, e);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) e[j] = T(-INFINITY);
+                }
+                clean(e);
+                f(v, e);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+    };
+
+    float top = -INFINITY;
+    if constexpr (STAGED) {
+#pragma unroll 4
+        for (int v = v0 + lane; v < v1; v += 32) {
+            alignas(16) T e[VE];
+            load(v, e);
+            clean(e);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) top = fmaxf(top, to_float(e[j]));
+            *reinterpret_cast<uint4*>(s_x + v * VE) = *reinterpret_cast<const uint4*>(e);
+        }
+    } else {
+        scan_range([&](int, const T (&e)[VE]) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) top = fmaxf(top, to_float(e[j]));
+        });
     }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
     if (lane == 0) sh.warp_max[warp] = top;
-    if (tid < SAMPLE_TABLE) sh.power[tid] = exp2((double)tid / SAMPLE_TABLE);
+    if (tid < SAMPLE_TABLE) sh.power[tid] = exp2(-(double)tid / SAMPLE_TABLE);
     for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.count[b] = 0;
     __syncthreads();
     top = sh.warp_max[lane & (SAMPLE_WARPS - 1)];
@@ -160,7 +263,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         if (tid == 0) sh.top = top;
         everywhere();
 #pragma unroll
-        for (int r = 0; r < C; ++r) top = fmaxf(top, *of_rank(&sh.top, r));
+        for (int r = 0; r < C; ++r) top = fmaxf(top, read(&sh.top, r));
     }
 
     if (top == -INFINITY) {   // nothing to draw
@@ -168,11 +271,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         everywhere();         // no CTA leaves while another may read its memory
         return;
     }
-    const bool infinite = top == INFINITY;
-    if (infinite) {           // infinite logits share the draw: they become zeros, everything else is out
-        for (int i = lane; i < held; i += 32) mine[i] = to_float(mine[i]) == INFINITY ? T(0.f) : T(-INFINITY);
-        __syncwarp();
+    if (top == INFINITY) {
+        infinite = true;
         top = 0.f;
+        if constexpr (STAGED) {
+            for (int v = v0 + lane; v < v1; v += 32) clean(*reinterpret_cast<T(*)[VE]>(s_x + v * VE));
+            __syncwarp();
+        }
     }
 
     double temperature = p.temperature_row ? (double)p.temperature_row[row] : p.temperature;
@@ -184,30 +289,43 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         temperature = 1.0;
     }
     temperature = fmin(temperature, 1e30);   // differences of logits that leave FP32 weigh nothing at any temperature
+    // An entry lies t = (top - v) * slope table steps below the largest, n of them to the nearest whole number or next to it:
+    // n from FP32 (of entries too far to weigh anything: from SAMPLE_FAR), the rest t - n from FP64.
     const double slope = 1.4426950408889634 * SAMPLE_TABLE / temperature;      // table steps per unit of logit
-    const float bin_slope = (float)(slope * ((double)SAMPLE_BINS / (SAMPLE_RANGE * SAMPLE_TABLE)));
+    const float slope_f = (float)slope, far = SAMPLE_FAR * SAMPLE_TABLE / slope_f;
     const double reach = min_p > 0.0 ? fmax(0.0, -log2(min_p)) * SAMPLE_TABLE : INFINITY;   // table steps that min-p leaves
-    const auto steps_below = [&](float v) { return ((double)top - (double)v) * slope; };
-    const auto weight = [&](float v) -> u64 {
-        const double t = steps_below(v);
-        return t < (double)(SAMPLE_RANGE * SAMPLE_TABLE) ? fixed_power(t, sh.power) : 0ull;
+    const auto steps_below = [&](float v) SAMPLE_INLINE { return ((double)top - (double)v) * slope; };
+    const auto whole_steps = [&](float v) SAMPLE_INLINE {
+        // a sum with 1.5 * 2^23 is rounded to a whole number
+        return __float_as_int(fmaf(fminf(top - v, far), slope_f, 12582912.f)) - __float_as_int(12582912.f);
     };
-    const auto bin_of = [&](float v) { return min(SAMPLE_BINS - 1, __float2int_rz((top - v) * bin_slope)); };
+    const auto weight_at = [&](float v, int n) SAMPLE_INLINE -> u64 {
+        const double whole = __hiloint2double(0x43380000, n) - 6755399441055744.0;   // 1.5 * 2^52 + n, less that
+        const u64 w = fixed_power(n, fma((double)top - (double)v, slope, -whole), sh.power);
+        return n < SAMPLE_RANGE * SAMPLE_TABLE ? w : 0ull;
+    };
+    const auto weight = [&](float v) SAMPLE_INLINE -> u64 { return weight_at(v, whole_steps(v)); };
+    const auto bin_of = [&](float v) SAMPLE_INLINE { return whole_steps(v) >> SAMPLE_BIN_BITS; };
 
-    // Every vector of a warp's range, before anything is moved.
-    const auto each_loaded = [&](auto&& f) {
-        for (int v = v0 + lane; v < v1; v += 32) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(s_x + v * VE);
-            const T* e = reinterpret_cast<const T*>(&raw);
+    float cut = -INFINITY;   // entries under it were dropped
+    // Every entry of the warp's range, before anything is moved.
+    const auto each_loaded = [&](auto&& f) SAMPLE_INLINE {
+        scan_range([&](int, const T (&e)[VE]) {
 #pragma unroll
             for (int j = 0; j < VE; ++j) f(to_float(e[j]));
-        }
+        });
     };
     // Every entry that is left.
-    const auto each = [&](auto&& f) {
-        for (int i = lane; i < held; i += 32) f(to_float(mine[i]));
+    const auto each = [&](auto&& f) SAMPLE_INLINE {
+        if (here) {
+            for (int i = lane; i < held; i += 32) f(to_float(mine[i]));
+        } else {
+            each_loaded([&](float v) {
+                if (v >= cut) f(v);
+            });
+        }
     };
-    const auto block_sum = [&](u64 v) {   // over the slice, to total_gt
+    const auto block_sum = [&](u64 v) SAMPLE_INLINE {   // over the slice, to total_gt
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
         if (lane == 0) sh.warp_sum[warp] = v;
@@ -219,7 +337,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         }
     };
     // The sums of the CTA's groups of bins, then a barrier of the row: what find() reads.
-    const auto publish = [&](bool counts, bool masses) {
+    const auto publish = [&](bool counts, bool masses) SAMPLE_INLINE {
         __syncthreads();
 #pragma unroll
         for (int g = 2 * warp; g < 2 * warp + 2; ++g) {
@@ -239,7 +357,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     // The bin of which `hit` says, by the running sum before and behind it, that it is the one (-1: none), with its entries and
     // the sum before it.  of(bins) and of(groups) give a lane's sum of the whole row.  The first warp looks, groups first:
     // reading every bin of every CTA took 5 us.
-    const auto find = [&](u64 carried, auto&& group_sum, auto&& bin_sum, auto&& hit) {
+    const auto find = [&](u64 carried, auto&& group_sum, auto&& bin_sum, auto&& hit) SAMPLE_INLINE {
         if (warp == 0) {
             int found = -1;
             u64 before = carried;
@@ -264,7 +382,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                 found = level == 0 ? l : found * 32 + l;
                 before = __shfl_sync(0xffffffffu, sum - own, l);
             }
-            if (found >= 0 && lane < C) entries = *of_rank(&sh.count[found], lane);
+            if (found >= 0 && lane < C) entries = read(&sh.count[found], lane);
             entries = __reduce_add_sync(0xffffffffu, entries);
             if (lane == 0) {
                 sh.bin = found;
@@ -274,48 +392,57 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         }
         everywhere();   // found, and no CTA clears what another still reads
     };
-    const auto group_counts = [&](int g) {
+    const auto group_counts = [&](int g) SAMPLE_INLINE {
         u64 c = 0;
 #pragma unroll
-        for (int r = 0; r < C; ++r) c += *of_rank(&sh.group_count[g], r);
+        for (int r = 0; r < C; ++r) c += read(&sh.group_count[g], r);
         return c;
     };
-    const auto counts = [&](int b) {
+    const auto counts = [&](int b) SAMPLE_INLINE {
         u64 c = 0;
 #pragma unroll
-        for (int r = 0; r < C; ++r) c += *of_rank(&sh.count[b], r);
+        for (int r = 0; r < C; ++r) c += read(&sh.count[b], r);
         return c;
     };
-    const auto group_masses = [&](int g) {
+    const auto group_masses = [&](int g) SAMPLE_INLINE {
         u64 m = 0;
 #pragma unroll
-        for (int r = 0; r < C; ++r) m += *of_rank(&sh.group_mass[g], r);
+        for (int r = 0; r < C; ++r) m += read(&sh.group_mass[g], r);
         return m;
     };
-    const auto masses = [&](int b) {
+    const auto masses = [&](int b) SAMPLE_INLINE {
         u64 m = 0;
 #pragma unroll
-        for (int r = 0; r < C; ++r) m += *of_rank(&sh.mass[b], r);
+        for (int r = 0; r < C; ++r) m += read(&sh.mass[b], r);
         return m;
     };
-    const auto clear = [&]() {
+    const auto clear = [&]() SAMPLE_INLINE {
         for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
             sh.count[b] = 0;
             sh.mass[b] = 0;
         }
         __syncthreads();
     };
-    // Which entries of a vector lie in the bins up to `bin`.
-    const auto in_front = [&](const T (&e)[VE], int bin) {
+    // The smallest number that lies in the bins up to `bin`, by a search of the warp over the order of the numbers' bits.
+    const auto end_of_bin = [&](int bin) SAMPLE_INLINE {
+        unsigned low = order_bits(-3.402823466e38f), high = order_bits(top);
+        while (low < high) {
+            const unsigned step = (high - low + 31) / 32, at = min(high, low + step * lane);
+            const int l = __ffs(__ballot_sync(0xffffffffu, bin_of(from_order_bits(at)) <= bin)) - 1;   // the largest number always is
+            if (l < 0) { low = min(high, low + step * 31 + 1); continue; }
+            high = min(high, low + step * l);
+            low = l == 0 ? high : low + step * (l - 1) + 1;
+        }
+        return from_order_bits(high);
+    };
+    // Which entries of a vector are not under the cut.
+    const auto in_front = [&](const T (&e)[VE]) SAMPLE_INLINE {
         unsigned stays = 0;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            const float f = to_float(e[j]);
-            if (f > -INFINITY && bin_of(f) <= bin) stays |= 1u << j;   // a NaN is not
-        }
+        for (int j = 0; j < VE; ++j) stays |= (to_float(e[j]) >= cut ? 1u : 0u) << j;   // a NaN is not
         return stays;
     };
-    const auto prefix = [&](int n, int& all) {   // over the lanes in front
+    const auto prefix = [&](int n, int& all) SAMPLE_INLINE {   // over the lanes in front
         int upto = n;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -325,38 +452,45 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         all = __shfl_sync(0xffffffffu, upto, 31);
         return upto - n;
     };
-    // Walks over the warp's range: f(vector, its entries up to `bin`, how many of them are in front of the vector's).
-    const auto walk = [&](int bin, auto&& f) {
+    // Walks over the warp's range: f(vector, its entries that stay, how many of them are in front of the vector's).
+    const auto walk = [&](auto&& f) SAMPLE_INLINE {
         int kept = 0;
-        for (int base = v0; base < v1; base += 32) {
-            const int v = base + lane;
-            alignas(16) T e[VE];
-            unsigned stays = 0;
-            if (v < v1) {
-                *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(s_x + v * VE);
-                stays = in_front(e, bin);
-            }
+        scan_range([&](int v, const T (&e)[VE]) {
+            const unsigned stays = in_front(e);
+            if (!__any_sync(0xffffffffu, stays)) return;
             int all;
             const int at = kept + prefix(__popc(stays), all);
             f(v, e, stays, at);
             kept += all;
             __syncwarp();
-        }
+        });
         return kept;
     };
-    int last = SAMPLE_BINS;   // the last bin that was kept
-    // Counts what lies in the bins up to `bin`.  Few entries go to the first CTA: true, and sh.mass there holds their keys
-    // (ordered by logit, then by place), sh.count their indices.  More move to the front of their warp's range, in order.
+    // Drops what lies behind `bin`.  Few entries go to the first CTA: true, and sh.mass there holds their keys (ordered by
+    // logit, then by place), sh.count their indices.  More move to the front of their warp's range, in order, or into its
+    // list.
     unsigned listed = 0;
-    const auto keep_up_to = [&](int bin) {
-        last = bin;
-        unsigned n = 0;
-        for (int v = v0 + lane; v < v1; v += 32) {
-            alignas(16) T e[VE];
-            *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(s_x + v * VE);
-            n += __popc(in_front(e, bin));
+    const auto keep_up_to = [&](int bin) SAMPLE_INLINE {
+        cut = end_of_bin(bin);
+        int n = 0;
+        if constexpr (STAGED) {
+            scan_range([&](int, const T (&e)[VE]) { n += __popc(in_front(e)); });
+            n = __reduce_add_sync(0xffffffffu, n);
+        } else {
+            n = walk([&](int v, const T (&e)[VE], unsigned stays, int at) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j)
+                    if (stays >> j & 1) {
+                        if (at < p.list) {
+                            places[at] = (unsigned short)((v - v0) * VE + j);
+                            mine[at] = e[j];
+                        }
+                        ++at;
+                    }
+            });
+            here = n <= p.list;   // else the range stays where it is
+            held = n;
         }
-        n = __reduce_add_sync(0xffffffffu, n);
         if (lane == 0) sh.warp_eq[warp] = n;
         __syncthreads();
         unsigned in_warps = lane < SAMPLE_WARPS ? sh.warp_eq[lane] : 0;
@@ -364,33 +498,33 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         in_warps = __reduce_add_sync(0xffffffffu, in_warps);
         if (tid == 0) sh.kept = in_warps;
         everywhere();
-        const unsigned in_slices = lane < C ? *of_rank(&sh.kept, lane) : 0;
+        const unsigned in_slices = lane < C ? read(&sh.kept, lane) : 0;
         const unsigned before_slice = __reduce_add_sync(0xffffffffu, lane < rank ? in_slices : 0);
         listed = __reduce_add_sync(0xffffffffu, in_slices);
-        if (listed > SAMPLE_THREADS) {
-            held = walk(bin, [&](int, const T (&e)[VE], unsigned stays, int at) {
+        const bool few = listed <= SAMPLE_THREADS;
+        const auto list = [&](unsigned place, float v, int index) SAMPLE_INLINE {
+            write(&sh.mass[place], 0, (u64)order_bits(v) << 32 | (0xffffffffu - place));
+            write(&sh.count[place], 0, (unsigned)index);
+        };
+        if constexpr (STAGED) {
+            held = walk([&](int v, const T (&e)[VE], unsigned stays, int at) {
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < VE; ++j)
-                    if (stays >> j & 1) mine[at++] = e[j];   // never ahead of what the warp has read
+                    if (stays >> j & 1) {
+                        if (few) list(before_slice + before_warp + at, to_float(e[j]), first + v * VE + j - shift);
+                        else mine[at] = e[j];   // never ahead of what the warp has read
+                        ++at;
+                    }
             });
-            return false;
+        } else if (few) {   // 512 at most: they are in the lists
+            for (int i = lane; i < held; i += 32)
+                list(before_slice + before_warp + i, to_float(mine[i]), first + v0 * VE + places[i] - shift);
         }
-        u64* keys = of_rank(sh.mass, 0);
-        unsigned* indices = of_rank(sh.count, 0);
-        walk(bin, [&](int v, const T (&e)[VE], unsigned stays, int at) {
-            unsigned place = before_slice + before_warp + at;
-#pragma unroll
-            for (int j = 0; j < VE; ++j)
-                if (stays >> j & 1) {
-                    keys[place] = (u64)order_bits(to_float(e[j])) << 32 | (0xffffffffu - place);
-                    indices[place++] = first + v * VE + j - shift;
-                }
-        });
-        everywhere();
-        return true;
+        if (few) everywhere();
+        return few;
     };
-    const auto block_scan = [&](u64 v, u64& all) {   // sum of the threads up to this one, and of all
+    const auto block_scan = [&](u64 v, u64& all) SAMPLE_INLINE {   // sum of the threads up to this one, and of all
         u64 sum = v;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -407,36 +541,41 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         }
         return sum;
     };
-    const auto uniform_part = [&](u64 all) {   // the whole part of u times the sum
+    const auto uniform_part = [&](u64 all) SAMPLE_INLINE {   // the whole part of u times the sum
         const float u = p.uniform[row];
         const double clipped = u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0;   // a NaN counts as zero
         return __umul64hi(all, (u64)(clipped * 0x1p64));
     };
+    // The threads' keys in descending order, over as many threads as `n` needs (a power of two), zeros behind: a bitonic
+    // network, inside a warp by shuffles and between warps through `scratch`.
+    const auto sort_down = [&](auto key, unsigned n, auto* scratch) SAMPLE_INLINE {
+        const int size_all = n > 1 ? 1 << (32 - __clz((int)n - 1)) : 1;
+        const bool active = warp * 32 < size_all;
+        for (int size = 2; size <= size_all; size <<= 1)
+            for (int j = size >> 1; j > 0; j >>= 1) {
+                auto other = key;
+                if (j >= 32) {
+                    __syncthreads();
+                    if (active) scratch[tid] = key;
+                    __syncthreads();
+                    if (active) other = scratch[tid ^ j];
+                } else if (active) {
+                    other = __shfl_xor_sync(0xffffffffu, key, j);
+                }
+                const bool larger = ((tid & size) == 0) == ((tid & j) == 0);
+                if (larger ? other > key : other < key) key = other;
+            }
+        return key;
+    };
     // The rest of the row's work where few candidates are left, by the first CTA: one a thread, sorted by logit and place.
-    const auto draw_from_list = [&](unsigned k, bool by_p, double target, bool sum_first) {
+    const auto draw_from_list = [&](unsigned k, bool by_p, double target, bool sum_first) SAMPLE_INLINE {
         if (rank != 0) return;
         u64 key = tid < (int)listed ? sh.mass[tid] : 0ull;
-        if (k < listed || by_p) {
-            for (int size = 2; size < 2 * (int)listed; size <<= 1)
-                for (int j = size >> 1; j > 0; j >>= 1) {
-                    u64 other;
-                    if (j >= 32) {
-                        __syncthreads();
-                        sh.mass[tid] = key;
-                        __syncthreads();
-                        other = sh.mass[tid ^ j];
-                    } else {
-                        other = __shfl_xor_sync(0xffffffffu, key, j);
-                    }
-                    const bool larger = ((tid & size) == 0) == ((tid & j) == 0);
-                    if (larger ? other > key : other < key) key = other;
-                }
-        }
+        if (k < listed || by_p) key = sort_down(key, listed, sh.mass);
         const unsigned place = 0xffffffffu - (unsigned)key;
         const float v = from_order_bits((unsigned)(key >> 32));
-        const double t = steps_below(v);
-        const u64 w = tid < (int)listed && tid < (int)k && t < (double)(SAMPLE_RANGE * SAMPLE_TABLE) ? fixed_power(t, sh.power) : 0ull;
-        bool stays = w != 0 && t <= reach;
+        const u64 w = tid < (int)listed && tid < (int)k ? weight(v) : 0ull;
+        bool stays = w != 0 && steps_below(v) <= reach;
         if (by_p) {
             u64 all;
             const u64 upto = block_scan(w, all);
@@ -456,29 +595,104 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
 
     // what stays: logits above `edge`, and the first `ties` of those on it
     float edge = -INFINITY;
-    unsigned ties = 0, on_edge = 0;
+    unsigned ties = 0;
 
-    // The border inside the bin that sh.bin names, among entries of which in_bin says whether they are in it.  By weight, a
-    // running sum reaches `target`; by count, it reaches `count`.
-    const auto refine = [&](bool by_mass, unsigned count, double target) {
-        const int bin = sh.bin;
+    // The border inside the bin `step`, on the edge of what a running sum reaches: of weights, `target`; of counts, `count`.
+    // `before` is that sum over the bins in front; with `sum_front` it is added up here.
+    // False: the border is in front of the step.
+    const auto refine = [&](int step, bool by_mass, unsigned count, double target, u64 before, bool sum_front) SAMPLE_INLINE {
+        u64 front = 0;
+        unsigned n = 0;
+        each([&](float v) {
+            const int b = bin_of(v);
+            if (b == step) n += v > -INFINITY && !(v < edge);
+            else if (sum_front && b < step) front += weight(v);
+        });
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) sh.warp_eq[warp] = n;
+        if (sum_front) block_sum(front);
+        else __syncthreads();
+        unsigned in_warps = lane < SAMPLE_WARPS ? sh.warp_eq[lane] : 0;
+        const unsigned before_warp = __reduce_add_sync(0xffffffffu, lane < warp ? in_warps : 0);
+        in_warps = __reduce_add_sync(0xffffffffu, in_warps);
+        if (tid == 0) sh.in_step = in_warps;
+        everywhere();
+        const unsigned in_slices = lane < C ? read(&sh.in_step, lane) : 0;
+        const unsigned before_slice = __reduce_add_sync(0xffffffffu, lane < rank ? in_slices : 0);
+        const unsigned all = __reduce_add_sync(0xffffffffu, in_slices);
+        if (sum_front)
+            for (int r = 0; r < C; ++r) before += read(&sh.total_gt, r);
+        if (sum_front && !((double)before < target)) {
+            everywhere();   // in_step and total_gt have been read
+            return false;
+        }
+        if (all <= SAMPLE_THREADS) {
+            // every CTA gets all entries of the step and sorts them
+            unsigned at = before_slice + before_warp;
+            for (int i0 = 0; i0 < (here ? held : 0); i0 += 32) {
+                const float v = i0 + lane < held ? to_float(mine[i0 + lane]) : -INFINITY;
+                const bool in = v > -INFINITY && !(v < edge) && bin_of(v) == step;
+                const unsigned lanes = __ballot_sync(0xffffffffu, in);
+                if (in)
+                    for (int r = 0; r < C; ++r) write(&sh.count[at + __popc(lanes & ((1u << lane) - 1))], r, order_bits(v));
+                at += __popc(lanes);
+            }
+            if (!here)
+                scan_range([&](int, const T (&e)[VE]) {
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) {
+                        const float v = to_float(e[j]);
+                        const bool in = v > -INFINITY && !(v < edge) && bin_of(v) == step;
+                        const unsigned lanes = __ballot_sync(0xffffffffu, in);
+                        if (in)
+                            for (int r = 0; r < C; ++r) write(&sh.count[at + __popc(lanes & ((1u << lane) - 1))], r, order_bits(v));
+                        at += __popc(lanes);
+                    }
+                });
+            everywhere();
+            const unsigned key = sort_down(tid < all ? sh.count[tid] : 0u, all, sh.count);
+            bool is_it = by_mass ? false : tid == count - 1 - (unsigned)before;
+            if (by_mass) {
+                const u64 w = tid < all ? weight(from_order_bits(key)) : 0ull;
+                u64 sum;
+                const u64 upto = before + block_scan(w, sum);
+                is_it = (double)(upto - w) < target && !((double)upto < target);
+            }
+            if (is_it) {
+                sh.edge = from_order_bits(key);
+                sh.ties = tid;
+            }
+            __syncthreads();
+            edge = sh.edge;
+            ties = __syncthreads_count(tid <= sh.ties && from_order_bits(key) == edge && tid < all);
+            everywhere();   // sh.count may be used again
+            return true;
+        }
         unsigned low = 0xffffffffu, high = 0;
         each([&](float v) {
-            if (bin_of(v) != bin || !(v > -INFINITY) || v < edge) return;
+            if (bin_of(v) != step || !(v > -INFINITY) || v < edge) return;
             const unsigned k = order_bits(v);
             low = min(low, k);
             high = max(high, k);
         });
         low = __reduce_min_sync(0xffffffffu, low);
         high = __reduce_max_sync(0xffffffffu, high);
-        if (tid == 0) { sh.low = 0xffffffffu; sh.high = 0; }
+        if (tid == 0) {
+            sh.low = 0xffffffffu;
+            sh.high = 0;
+            sh.bin_count = all;
+            sh.before = before;
+        }
         __syncthreads();
-        if (lane == 0) { atomicMin(&sh.low, low); atomicMax(&sh.high, high); }
+        if (lane == 0) {
+            atomicMin(&sh.low, low);
+            atomicMax(&sh.high, high);
+        }
         everywhere();
 #pragma unroll
         for (int r = 0; r < C; ++r) {
-            low = min(low, *of_rank(&sh.low, r));
-            high = max(high, *of_rank(&sh.high, r));
+            low = min(low, read(&sh.low, r));
+            high = max(high, read(&sh.high, r));
         }
         while (low != high) {
             const int width = 32 - __clz(high - low), down = width > 10 ? width - 10 : 0;   // 1024 bins
@@ -488,11 +702,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                 const unsigned k = order_bits(v);
                 if (k < low || k > high) return;
                 const int b = (int)((high - k) >> down);
-                if (by_mass) {
-                    const u64 w = weight(v);
-                    if (w == 0) return;
-                    atomicAdd(&sh.mass[b], w);
-                }
+                if (by_mass) atomicAdd(&sh.mass[b], weight(v));
                 atomicAdd(&sh.count[b], 1u);
             });
             publish(true, by_mass);
@@ -504,34 +714,31 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             low = down == 0 ? high : max(low, high - ((1u << down) - 1));
         }
         edge = from_order_bits(high);
-        on_edge = sh.bin_count;
+        ties = count - (unsigned)sh.before;
         if (by_mass) {
-            const u64 w = weight(edge), before = sh.before;
-            unsigned keep = 1;
-            const double want = (target - (double)before) / (double)w;
-            if (want > 1.0) keep = (unsigned)fmin(ceil(want), (double)on_edge);
-            while (keep > 1 && !((double)(before + (keep - 1) * w) < target)) --keep;
-            while (keep < on_edge && (double)(before + keep * w) < target) ++keep;
-            ties = keep;
-        } else {
-            ties = count - (unsigned)sh.before;
+            const u64 w = weight(edge), in_front_of = sh.before;
+            const unsigned equal = sh.bin_count;
+            ties = (unsigned)fmin(fmax(ceil((target - (double)in_front_of) / (double)w), 1.0), (double)equal);
+            while (ties > 1 && !((double)(in_front_of + (ties - 1) * w) < target)) --ties;
+            while (ties < equal && (double)(in_front_of + ties * w) < target) ++ties;
         }
-        __syncthreads();   // sh.before and sh.bin_count are read by everyone before they change
+        everywhere();   // sh.before and sh.bin_count are read by everyone before they change
+        return true;
     };
 
-    const int min_p_bin = reach < SAMPLE_RANGE * SAMPLE_TABLE ? (int)(reach * ((double)SAMPLE_BINS / (SAMPLE_RANGE * SAMPLE_TABLE))) + 1 : SAMPLE_BINS;
+    const int min_p_bin = reach < SAMPLE_RANGE * SAMPLE_TABLE ? ((int)reach >> SAMPLE_BIN_BITS) + 1 : SAMPLE_BINS;
     const bool by_k = top_k > 1 && top_k < p.V, by_p = top_k != 1 && top_p < 1.0;
     double target = 0.0;
+    // the borders still to be found: of top-k, of top-p at the end of what is left, of top-p anywhere in what is left
+    enum { DONE, TOP_K, TOP_P, TOP_P_LEFT };
     if (top_k == 1) {
         // the first entry that equals the largest
         unsigned at = 0xffffffffu;
-        for (int v = v0 + lane; v < v1; v += 32) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(s_x + v * VE);
-            const T* e = reinterpret_cast<const T*>(&raw);
+        scan_range([&](int v, const T (&e)[VE]) {
 #pragma unroll
             for (int j = VE - 1; j >= 0; --j)
                 if (to_float(e[j]) == top) at = min(at, (unsigned)(first + v * VE + j - shift));
-        }
+        });
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) sh.warp_eq[warp] = at;
         __syncthreads();
@@ -541,89 +748,98 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         }
         everywhere();
         if (rank == 0 && warp == 0) {
-            at = __reduce_min_sync(0xffffffffu, *of_rank(&sh.low, lane & (C - 1)));
+            at = __reduce_min_sync(0xffffffffu, read(&sh.low, lane & (C - 1)));
             if (lane == 0) p.tokens[row] = at;
         }
         everywhere();   // no CTA leaves while another may read its memory
         return;
     }
+    int step = 0, keep = SAMPLE_BINS;   // the step of the first rule's border, and the last bin that is kept
+    int rule = DONE;
     if (by_k) {
         each_loaded([&](float v) {
             if (v > -INFINITY) atomicAdd(&sh.count[bin_of(v)], 1u);
         });
         publish(true, false);
         find(0, group_counts, counts, [&](u64 a, u64 b) { return a < (unsigned)top_k && b >= (unsigned)top_k; });
-        const int bin = sh.bin;   // -1: fewer candidates than top-k keeps
-        const int limit = bin < 0 ? SAMPLE_BINS - 1 : bin;
-        const bool cut = !by_p && min_p_bin < limit;   // by min-p: all that is in front of that is among the first k
-        if (keep_up_to(cut ? min_p_bin : limit)) {
-            draw_from_list((unsigned)top_k, by_p, 0.0, true);
-            return;
-        }
-        if (!cut && bin >= 0) refine(false, (unsigned)top_k, 0.0);
-        if (by_p) {   // the weight of what top-k keeps
-            u64 sum = 0;
-            each([&](float v) { if (v > edge) sum += weight(v); });
-            block_sum(sum);
-            everywhere();
-            u64 all = edge > -INFINITY ? ties * weight(edge) : 0ull;
-            for (int r = 0; r < C; ++r) all += *of_rank(&sh.total_gt, r);
-            target = top_p * (double)all;
-        }
+        step = sh.bin;   // -1: fewer candidates than top-k keeps
+        keep = step < 0 ? SAMPLE_BINS - 1 : step;
+        if (!by_p && min_p_bin < keep) keep = min_p_bin;   // all that is in front of that is among the first k
+        else if (step >= 0) rule = TOP_K;
+        if (by_p && rule == DONE) rule = TOP_P_LEFT;
     } else if (by_p) {
         // the sum of all weights, and a histogram of their upper 16 bits (relative to the largest of the bin): its running
         // sums are not above the true ones, so the border is not behind the bin in which they reach the target
-        const auto bin_shift = [](int b) { return max(0, SAMPLE_WEIGHT_BITS - 15 - b * SAMPLE_RANGE / SAMPLE_BINS); };
+        constexpr int PER_BINADE = SAMPLE_TABLE >> SAMPLE_BIN_BITS;
+        const auto bin_shift = [](int b) { return max(0, SAMPLE_WEIGHT_BITS - 15 - b / PER_BINADE); };
         u64 sum = 0;
         each_loaded([&](float v) {
-            const u64 w = weight(v);
+            const int n = whole_steps(v), b = n >> SAMPLE_BIN_BITS;
+            const u64 w = weight_at(v, n);
             sum += w;
-            const int b = bin_of(v);
             if (w != 0) atomicAdd(&sh.count[b], (unsigned)(w >> bin_shift(b)));
         });
         block_sum(sum);
         for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.mass[b] = (u64)sh.count[b] << bin_shift(b);
         publish(false, true);
         u64 all = 0;
-        for (int r = 0; r < C; ++r) all += *of_rank(&sh.total_gt, r);
+        for (int r = 0; r < C; ++r) all += read(&sh.total_gt, r);
         target = top_p * (double)all;
         find(0, group_masses, masses, [&](u64 a, u64 b) { return (double)a < target && !((double)b < target); });
-        if (keep_up_to(min(sh.bin < 0 ? SAMPLE_BINS - 1 : sh.bin, min_p_bin))) {
-            draw_from_list(SAMPLE_THREADS, true, target, false);
-            return;
-        }
-    } else if (min_p_bin < SAMPLE_BINS) {
-        if (keep_up_to(min_p_bin)) {
-            draw_from_list(SAMPLE_THREADS, false, 0.0, false);
-            return;
-        }
+        step = sh.bin < 0 ? SAMPLE_BINS - 1 : sh.bin;
+        keep = min(step, min_p_bin);
+        if (step <= min_p_bin) rule = TOP_P;   // else min-p cuts in front of the border
+    } else {
+        keep = min_p_bin;
     }
-    if (by_p) {
-        clear();
-        each([&](float v) {
-            const u64 w = weight(v);
-            if (w == 0 || v < edge) return;
-            const int b = bin_of(v);
-            atomicAdd(&sh.mass[b], w);
-            atomicAdd(&sh.count[b], 1u);
-        });
-        publish(true, true);
-        find(0, group_masses, masses, [&](u64 a, u64 b) { return (double)a < target && !((double)b < target); });
-        if (sh.bin >= 0) refine(true, 0, target);   // else min-p has cut in front of the border
+    const u64 in_front_of_step = sh.before;
+    if (keep < SAMPLE_BINS && keep_up_to(keep)) {
+        draw_from_list(by_k ? (unsigned)top_k : SAMPLE_THREADS, by_p, target, by_k);
+        return;
+    }
+    while (rule != DONE) {
+        if (rule == TOP_P_LEFT) {
+            if (by_k) {   // the weight of what top-k keeps
+                u64 sum = 0;
+                each([&](float v) { if (v > edge) sum += weight(v); });
+                block_sum(sum);
+                everywhere();
+                u64 all = edge > -INFINITY ? ties * weight(edge) : 0ull;
+                for (int r = 0; r < C; ++r) all += read(&sh.total_gt, r);
+                target = top_p * (double)all;
+            }
+            clear();
+            each([&](float v) {
+                const u64 w = weight(v);
+                if (w == 0 || v < edge) return;
+                const int b = bin_of(v);
+                atomicAdd(&sh.mass[b], w);
+                atomicAdd(&sh.count[b], 1u);
+            });
+            publish(true, true);
+            find(0, group_masses, masses, [&](u64 a, u64 b) { return (double)a < target && !((double)b < target); });
+            step = sh.bin;
+        }
+        const bool found = refine(step, rule != TOP_K, (unsigned)top_k, target, rule == TOP_K ? in_front_of_step : rule == TOP_P ? 0 : sh.before,
+                                  rule == TOP_P);
+        rule = rule == TOP_K && by_p ? TOP_P_LEFT : rule == TOP_P && !found ? TOP_P_LEFT : DONE;
     }
 
     // the draw
-    const auto drawn_weight = [&](float v) -> u64 {
-        const double t = steps_below(v);
-        return t <= reach && t < (double)(SAMPLE_RANGE * SAMPLE_TABLE) ? fixed_power(t, sh.power) : 0ull;
+    const auto drawn_weight = [&](float v) SAMPLE_INLINE -> u64 {
+        return reach == INFINITY || steps_below(v) <= reach ? weight(v) : 0ull;
     };
     const u64 edge_weight = edge > -INFINITY ? drawn_weight(edge) : 0ull;
     u64 gt = 0;
     unsigned eq = 0;
-    each([&](float v) {
-        if (v > edge) gt += drawn_weight(v);
-        else if (v == edge) ++eq;
-    });
+    if (cut == -INFINITY) {   // no rule: no border either
+        each_loaded([&](float v) { gt += weight(v); });
+    } else {
+        each([&](float v) {
+            if (v > edge) gt += drawn_weight(v);
+            else if (v == edge) ++eq;
+        });
+    }
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) sh.warp_eq[warp] = eq;
     block_sum(gt);
@@ -636,8 +852,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     u64 all = 0, before = 0, own = 0;
     unsigned seen = 0, passed = 0;   // candidates on the edge before this slice, then before this warp
     for (int r = 0; r < C; ++r) {
-        const unsigned e = *of_rank(&sh.total_eq, r), keep = passed < ties ? min(e, ties - passed) : 0;
-        const u64 sum = *of_rank(&sh.total_gt, r) + keep * edge_weight;
+        const unsigned e = read(&sh.total_eq, r), keep = passed < ties ? min(e, ties - passed) : 0;
+        const u64 sum = read(&sh.total_gt, r) + keep * edge_weight;
         if (r == rank) {
             before = all;
             own = sum;
@@ -656,6 +872,50 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     }
     own = sh.warp_sum[warp] + (seen < ties ? min(sh.warp_eq[warp], ties - seen) : 0) * edge_weight;
     if (drawn < before || drawn >= before + own) return;   // another warp's
+    if (!here) {   // over the range itself, a vector a lane
+        bool done = false;
+        scan_range([&](int v, const T (&e)[VE]) {
+            if (done) return;
+            u64 sum = 0;
+            int on = 0;
+            const unsigned stays = in_front(e);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const float f = to_float(e[j]);
+                if (!(stays >> j & 1)) continue;
+                if (f > edge) sum += drawn_weight(f);
+                else if (f == edge && f > -INFINITY) ++on;
+            }
+            int on_all;
+            const unsigned ahead = seen + prefix(on, on_all);
+            sum += (ahead < ties ? min((unsigned)on, ties - ahead) : 0) * edge_weight;
+            u64 upto = sum;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const u64 o = __shfl_up_sync(0xffffffffu, upto, s);
+                if (lane >= s) upto += o;
+            }
+            const u64 from = before + upto - sum;
+            if (drawn >= from && drawn < from + sum) {
+                u64 run = from;
+                unsigned k = ahead;
+                for (int j = 0; j < VE; ++j) {
+                    const float f = to_float(e[j]);
+                    if (!(stays >> j & 1)) continue;
+                    if (f > edge) run += drawn_weight(f);
+                    else if (f == edge && f > -INFINITY && k++ < ties) run += edge_weight;
+                    if (run > drawn) {
+                        p.tokens[row] = first + v * VE + j - shift;
+                        break;
+                    }
+                }
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+            seen += on_all;
+            done = drawn < before;
+        });
+        return;
+    }
     int place = -1;   // of the token among what the warp holds
     for (int base = 0; base < held && place < 0; base += 32) {
         const int i = base + lane;
@@ -673,29 +933,39 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         before += __shfl_sync(0xffffffffu, sum, 31);
         seen += __popc(edge_lanes);
     }
-    if (last == SAMPLE_BINS) {   // nothing was moved
+    if (!STAGED) place = places[place];
+    if (!STAGED || cut == -INFINITY) {
         if (lane == 0) p.tokens[row] = first + v0 * VE + place - shift;
         return;
     }
     // the place-th of those entries of the warp's range that were kept, counted again in the row itself
-    for (int base = v0; base < v1; base += 32) {
-        const int v = base + lane;
-        unsigned stays = 0;
-        if (v < v1) {
-            alignas(16) T e[VE];
-            load(v, e);
-            if (infinite)
-                for (int j = 0; j < VE; ++j) e[j] = to_float(e[j]) == INFINITY ? T(0.f) : T(-INFINITY);
-            stays = in_front(e, last);
+    constexpr int AHEAD = 4;
+    for (int base = v0; base < v1; base += 32 * AHEAD) {
+        alignas(16) T e[AHEAD][VE];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (base + 32 * a + lane < v1) {
+                load(base + 32 * a + lane, e[a]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) e[a][j] = T(-INFINITY);
+            }
         }
-        int all_kept;
-        const int n = __popc(stays), from = prefix(n, all_kept);
-        if (place >= from && place < from + n)
-            for (int j = 0, k = from; j < VE; ++j)
-                if (stays >> j & 1 && k++ == place) p.tokens[row] = first + v * VE + j - shift;
-        if (place < all_kept) return;
-        place -= all_kept;
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            clean(e[a]);
+            const unsigned stays = in_front(e[a]);
+            int all_kept;
+            const int n = __popc(stays), from = prefix(n, all_kept);
+            if (place >= from && place < from + n)
+                for (int j = 0, k = from; j < VE; ++j)
+                    if (stays >> j & 1 && k++ == place) p.tokens[row] = first + (base + 32 * a + lane) * VE + j - shift;
+            if (place < all_kept) return;
+            place -= all_kept;
+        }
     }
 }
+
+#undef SAMPLE_INLINE
 
 }  // namespace sd

@@ -153,24 +153,33 @@ bool token_fuses(const sd_int8_linear_args* a) {
 size_t q_bytes(const sd_int8_linear_args* a) { return ((size_t)a->rows * padded(a->K) + 255) / 256 * 256; }
 
 // ---- sampling ----
-constexpr size_t SAMPLE_SLICE_BYTES = 96 * 1024;   // of a CTA, where eight CTAs a row are not too few
-constexpr size_t SAMPLE_SMEM = 132 * 1024;         // a slice of the largest vocabulary in FP32 over eight CTAs, and its alignment
-static_assert((SAMPLE_MAX_VOCAB / 8 + 8) * 4 <= SAMPLE_SMEM, "the largest slice");
+constexpr size_t SAMPLE_STAGED = 94 * 1024;     // bytes of a slice that is kept in shared memory: two CTAs share an SM
+constexpr size_t SAMPLE_LIST_BYTES = 60 * 1024;
+constexpr long long SAMPLE_L2 = 96 << 20;       // of 126 MB
+static_assert(2 * (SAMPLE_STAGED + sizeof(SampleShared) + 1024) <= 228 * 1024 &&
+              2 * (SAMPLE_RING_BYTES + SAMPLE_LIST_BYTES + sizeof(SampleShared) + 1024) <= 228 * 1024, "two CTAs an SM");
 template <class T, int C>
 int launch_sample(SampleParams p, long long rows, cudaStream_t stream) {
     constexpr int VE = 16 / sizeof(T);
     // rows may start up to VE - 1 elements behind a 16-byte boundary
     p.slice = ((p.V + VE - 1 + C - 1) / C + VE - 1) / VE * VE;
-    return launch<k_sample<T, C>>((unsigned)(rows * C), SAMPLE_THREADS, (size_t)p.slice * sizeof(T), SAMPLE_SMEM, C, false, stream, p);
+    const size_t bytes = (size_t)p.slice * sizeof(T);
+    if (bytes <= SAMPLE_STAGED)
+        return launch<k_sample<T, C, true>>((unsigned)(rows * C), SAMPLE_THREADS, bytes, SAMPLE_STAGED, C, false, stream, p);
+    p.list = SAMPLE_LIST_BYTES / SAMPLE_WARPS / (sizeof(T) + sizeof(unsigned short));
+    constexpr size_t smem = SAMPLE_RING_BYTES + SAMPLE_LIST_BYTES;
+    return launch<k_sample<T, C, false>>((unsigned)(rows * C), SAMPLE_THREADS, smem, smem, C, false, stream, p);
 }
 template <class T>
 int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
-    // as many CTAs a row as keep the SMs busy, with slices of 2048 entries at least and 96 KB at most
-    const auto fits = [&](int c) { return (size_t)p.V * sizeof(T) <= c * SAMPLE_SLICE_BYTES; };
-    const auto worth = [&](int c) { return rows * c <= 2 * 148 && p.V >= c * 2048; };
-    if (worth(8) || !fits(4)) return launch_sample<T, 8>(p, rows, stream);
-    if (worth(4) || !fits(2)) return launch_sample<T, 4>(p, rows, stream);
-    if (worth(2) || !fits(1)) return launch_sample<T, 2>(p, rows, stream);
+    // as many CTAs a row as the SMs take at once, two on each, with 2048 entries at least; and so many that the rows in work
+    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32: 376 us with one CTA, TODO with two)
+    const auto worth = [&](int c) {
+        return p.V >= c * 2048 && (rows * c <= 2 * 148 || 2 * 148 / (c / 2) * (long long)p.V * (int)sizeof(T) > SAMPLE_L2);
+    };
+    if (worth(8)) return launch_sample<T, 8>(p, rows, stream);
+    if (worth(4)) return launch_sample<T, 4>(p, rows, stream);
+    if (worth(2)) return launch_sample<T, 2>(p, rows, stream);
     return launch_sample<T, 1>(p, rows, stream);
 }
 

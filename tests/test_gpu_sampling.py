@@ -36,6 +36,20 @@ def test_every_rule_at_every_size(rows, vocab, dtype):
         _same(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
 
+@pytest.mark.parametrize("dtype,rows,vocab", ((torch.float32, 300, 26001), (torch.bfloat16, 310, 60003), (torch.float32, 160, 90000)))
+def test_rows_too_long_for_shared_memory(dtype, rows, vocab):
+    """Many rows of a large vocabulary: few candidates, some thousands, and nearly all of them stay."""
+    logits, u = _logits(rows, vocab, 11, dtype)
+    logits[::7, ::3] = -math.inf
+    logits[5] = -math.inf
+    logits[6, 100:] = math.nan
+    logits[9, 5], logits[9, vocab - 1] = math.inf, math.inf
+    logits[12] = 0.25
+    for settings in (dict(), dict(top_k=40, top_p=0.9), dict(top_k=3000), dict(top_k=vocab - 100, top_p=0.97), dict(top_p=0.9), dict(top_p=0.999, temperature=1.5),
+                     dict(min_p=0.05), dict(min_p=1e-4, top_p=0.99), dict(temperature=0.0), dict(top_p=0.3, temperature=30.0)):
+        _same(logits, u, **settings)
+
+
 def test_settings_of_each_row():
     logits, u = _logits(64, 3000, 3)
     gen = torch.Generator().manual_seed(1)
