@@ -5,6 +5,7 @@
 // zeros has scale 0; a row that holds an infinity or a NaN gets zeros and the scale NaN, so all its products are NaN.
 #pragma once
 #include <cuda_bf16.h>
+#include <type_traits>
 
 #include "sd_common.cuh"
 #include "sd_tc.cuh"
@@ -26,33 +27,42 @@ __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x
 
 // What a row's largest magnitude (its bits) makes of the row.
 struct RowScale {
-    float scale, inverse;   // a / 127 and about 127 / a
-    double largest;
-    bool tiny, bad;         // tiny: the inverse may overflow, every entry is taken in 64 bits
+    float scale, inverse, largest;   // a / 127, about 127 / a, a
+    bool bad, special;               // not finite; that, or so small that the inverse may overflow
 };
 __device__ __forceinline__ RowScale row_scale(unsigned largest_bits) {
     RowScale r;
-    const float a = __uint_as_float(largest_bits);
+    r.largest = __uint_as_float(largest_bits);
     r.bad = largest_bits >= 0x7f800000u;
-    r.scale = r.bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(a, 127.f);
-    r.tiny = a < 1e-30f;
-    r.inverse = r.tiny || r.bad ? 0.f : __fdiv_rn(127.f, a);
-    r.largest = a;
+    r.special = r.bad || r.largest < 1e-30f;
+    r.scale = r.bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(r.largest, 127.f);
+    r.inverse = r.special ? 0.f : __fdiv_rn(127.f, r.largest);
     return r;
 }
-// 127 x / a rounded to nearest even.  x times the rounded inverse is at most 1.5 * 2^-23 of itself off, under 2^-15: only
-// where that leaves open which side of a half the quotient is on, 127 x is compared with half * a, both exact in 64 bits.
-__device__ __forceinline__ int quantize_value(float x, const RowScale& r) {
-    if (r.bad || x == 0.f) return 0;
-    const float t = x * r.inverse;
-    float n = rintf(t);
-    if (r.tiny || fabsf(fabsf(t - n) - 0.5f) < 3.1e-5f) {
-        if (r.tiny) return (int)rint(127.0 * (double)x / r.largest);
-        const double half = floor((double)t * 2.0 + 0.5) * 0.5, exact = 127.0 * (double)x, border = half * r.largest;
-        const double low = floor(half), up = low + 1.0;   // half is the odd multiple of 1/2 next to t
-        n = (float)(exact > border ? up : exact < border ? low : (fmod(low, 2.0) == 0.0 ? low : up));
+// 127 x / a rounded to nearest even, where the product below leaves it open: 127 x is compared with half * a, both exact in
+// 64 bits.
+__device__ __noinline__ int quantize_exactly(float x, float inverse, float a) {
+    if (a < 1e-30f) return a == 0.f ? 0 : (int)rint(127.0 * (double)x / (double)a);
+    // the product is less than a half off, so the quotient lies between the neighbours of this half
+    const double low = floor((double)(x * inverse)), exact = 127.0 * (double)x, border = (low + 0.5) * (double)a;
+    return (int)(exact > border ? low + 1.0 : exact < border ? low : 2.0 * rint(low * 0.5 + 0.25));
+}
+// Four entries as bytes.  x times the rounded inverse is at most 1.5 * 2^-23 of itself off, under 2^-15; its sum with
+// 1.5 * 2^23 is the nearest whole number, in the low bits, unless it lies that close to a half.
+__device__ __forceinline__ unsigned quantize_four(const float* v, const RowScale& r) {
+    unsigned w[4];
+    float far = 0.f;   // from the whole numbers
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float t = v[e] * r.inverse, n = t + 12582912.f;
+        far = fmaxf(far, fabsf(t - (n - 12582912.f)));
+        w[e] = __float_as_uint(n);
     }
-    return (int)n;
+    if (r.special || far > 0.5f - 3.1e-5f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = r.bad ? 0u : (unsigned)quantize_exactly(v[e], r.inverse, r.largest);
+    }
+    return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
 }
 
 template <class T>
@@ -62,66 +72,81 @@ __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Eight entries of a row from column c0 on, zeros past its end.
+// Eight entries of a row from column c0 on, zeros past its end.  VEC: rows start on 16-byte boundaries and K is a multiple of
+// eight, so that a request is one predicated instruction and a lane's requests go out together.
 template <class T, bool VEC>
 __device__ __forceinline__ void load_eight(const T* row, int c0, int K, float (&v)[8]) {
-    if (VEC && c0 + 8 <= K) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(row + c0);
-            const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    if constexpr (!VEC) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = __bfloat1622float2(p[e]);
-                v[2 * e] = f.x;
-                v[2 * e + 1] = f.y;
-            }
-        } else {
-            const float4 a = *reinterpret_cast<const float4*>(row + c0), b = *reinterpret_cast<const float4*>(row + c0 + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        for (int e = 0; e < 8; ++e) v[e] = c0 + e < K ? to_float(row[c0 + e]) : 0.f;
+    } else if constexpr (sizeof(T) == 2) {
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        if (c0 < K) raw = *reinterpret_cast<const uint4*>(row + c0);
+        const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = __bfloat1622float2(p[e]);
+            v[2 * e] = f.x;
+            v[2 * e + 1] = f.y;
         }
-        return;
+    } else {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (c0 < K) {
+            a = *reinterpret_cast<const float4*>(row + c0);
+            b = *reinterpret_cast<const float4*>(row + c0 + 4);
+        }
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c0 + e < K ? to_float(row[c0 + e]) : 0.f;
 }
-__device__ __forceinline__ unsigned quantize_four(const float* v, const RowScale& r) {
-    unsigned w = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w |= (unsigned)(quantize_value(v[e], r) & 0xff) << (8 * e);
-    return w;
-}
-
-// One CTA per row: the row is read for its largest magnitude and again, then out of L1 or L2, for its entries.  q rows start
-// on 16-byte boundaries, q_stride covers K rounded up to 16, and the bytes past K are set to zero.
+// Groups of W warps take a row each, eight rows to W = 1 in a CTA; a lane keeps up to H pieces of eight entries between the
+// search for the largest magnitude and the rounding (longer rows are read again).  q rows start on 16-byte boundaries,
+// q_stride covers K rounded up to 16, and the bytes past K are set to zero.
 constexpr int QUANT_THREADS = 256;
-template <class T, bool VEC>
+template <class T, bool VEC, int W, int H>
 __global__ void __launch_bounds__(QUANT_THREADS) k_quantize_rows(QuantizeParams p) {
     __shared__ unsigned s_max[QUANT_THREADS / 32];
     chain_wait();
     chain_release();
-    const T* row = reinterpret_cast<const T*>(p.x) + (long long)blockIdx.x * p.x_stride;
+    const int warp = threadIdx.x >> 5, at = (warp % W) * 32 + (threadIdx.x & 31);
+    const long long r_idx = (long long)blockIdx.x * (8 / W) + warp / W;
+    const bool live = r_idx < p.rows;   // the rows of a CTA share its barrier
+    const T* row = reinterpret_cast<const T*>(p.x) + (live ? r_idx : 0) * p.x_stride;
+    float held[H][8];
     unsigned top = 0;
-    for (int c0 = threadIdx.x * 8; c0 < p.K; c0 += QUANT_THREADS * 8) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) load_eight<T, VEC>(row, (h * W * 32 + at) * 8, p.K, held[h]);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, abs_bits(held[h][e]));
+    for (int c0 = (H * W * 32 + at) * 8; c0 < p.K; c0 += W * 256) {
         float v[8];
         load_eight<T, VEC>(row, c0, p.K, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = s_max[threadIdx.x & (QUANT_THREADS / 32 - 1)];
-    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (W > 1) {
+        if ((threadIdx.x & 31) == 0) s_max[warp] = top;
+        __syncthreads();
+        top = __reduce_max_sync(0xffffffffu, s_max[warp / W * W + threadIdx.x % W]);
+    }
+    if (!live) return;
     const RowScale r = row_scale(top);
-    signed char* out = p.q + (long long)blockIdx.x * p.q_stride;
+    signed char* out = p.q + r_idx * p.q_stride;
     const int padded = (p.K + 15) / 16 * 16;
-    for (int c0 = threadIdx.x * 8; c0 < padded; c0 += QUANT_THREADS * 8) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const int c0 = (h * W * 32 + at) * 8;
+        if (c0 < padded) *reinterpret_cast<uint2*>(out + c0) = make_uint2(quantize_four(held[h], r), quantize_four(held[h] + 4, r));
+    }
+    for (int c0 = (H * W * 32 + at) * 8; c0 < padded; c0 += W * 256) {
         float v[8];
         load_eight<T, VEC>(row, c0, p.K, v);
         *reinterpret_cast<uint2*>(out + c0) = make_uint2(quantize_four(v, r), quantize_four(v + 4, r));
     }
-    if (threadIdx.x == 0) p.scale[blockIdx.x] = r.scale;
+    if (at == 0) p.scale[r_idx] = r.scale;
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
@@ -145,102 +170,155 @@ __device__ __forceinline__ float int8_bias(const Int8Params& p, int n) {
 // silu(gate) * value, both in FP32, rounded once by the store
 __device__ __forceinline__ float int8_gated(float gate, float value) { return gate * sigmoidf_(gate) * value; }
 
-// tcgen05.mma.kind::i8, int32 accumulators in tensor memory.  Per CTA: tiles of 128 rows by BN weight rows, both K-major
-// in shared memory as rows of 128 bytes with the 128-byte swizzle, loaded by TMA (which fills what lies outside with
-// zeros: ragged M, N and K need nothing else) into a ring of stages.  With SwiGLU the BN weight rows are BN / 2 gate rows
-// and the BN / 2 value rows that belong to them, so that one tile's accumulator holds both factors of its outputs.
+// tcgen05.mma.kind::i8, int32 accumulators in tensor memory, both operands K-major in shared memory as rows of 128 bytes with
+// the 128-byte swizzle, loaded by TMA (which fills what lies outside with zeros: ragged M, N and K need nothing else) into a
+// ring of stages.  Persistent: one thread loads, one issues the products, eight warps empty the accumulator, of which there
+// are two, so that the products of a tile run under the epilogue of the one before.  With SwiGLU half of a tile's weight rows
+// are gate rows and half the value rows that belong to them, so that its accumulator holds both factors of its outputs.
 //
-// One CTA per SM stays for all its tiles.  One thread loads, one thread issues the products, eight warps empty the
-// accumulator, of which there are two, so that the products of a tile run under the epilogue of the one before.
+// PAIR: two CTAs of a cluster share a tile of 256 rows by 256 weight rows (cta_group::2): each loads 128 of either, the first
+// one's thread issues for both, each holds 128 rows of the accumulator.  One CTA by itself with 128 x 256 moves 12 KB of
+// operands for an instruction of 128 clocks and receives as much, more than the 128 bytes a clock of its shared memory; a pair
+// moves 8 KB.  Without PAIR tiles are 128 rows by BN, for few rows or few tiles.
 constexpr int I8_BM = 128, I8_BK = 128, I8_THREADS = 384, I8_EPILOGUE_WARP = 4, I8_EPILOGUE_THREADS = 256;
 constexpr int I8_GROUP = 8;   // row tiles that are walked together: their rows and the weight tiles stay in L2
-template <int BN>
+constexpr int I8_STAGING = 32 * 64;   // bytes of a warp, see int8_store
+template <int BN, bool PAIR>
 struct Int8Tile {
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr unsigned A_BYTES = I8_BM * I8_BK, B_BYTES = BN * I8_BK, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // weight rows that a CTA loads
+    static constexpr unsigned A_BYTES = I8_BM * I8_BK, B_BYTES = B_ROWS * I8_BK, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 192 * 1024 / STAGE_BYTES;
     static constexpr unsigned TMEM_COLS = 2 * BN;
-    static constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + 1024;
+    static constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + 8 * I8_STAGING + 1024;
 };
 
-__device__ __forceinline__ void tc_load_2d(unsigned smem, const CUtensorMap* map, int col, int row, unsigned bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem),
-        "l"(reinterpret_cast<unsigned long long>(map)), "r"(col), "r"(row), "r"(bar)
-        : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void i8_load(unsigned smem, const CUtensorMap* map, int col, int row, unsigned bar) {
+    if constexpr (PAIR)   // the barrier may be the other CTA's
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem),
+            "l"(reinterpret_cast<unsigned long long>(map)), "r"(col), "r"(row), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem),
+            "l"(reinterpret_cast<unsigned long long>(map)), "r"(col), "r"(row), "r"(bar)
+            : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void i8_mma(unsigned d_tmem, unsigned long long da, unsigned long long db, unsigned idesc,
                                        unsigned accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
-// int32 accumulator (2 at bit 4), signed operands (1 at bits 7 and 10), both K-major, M = 128
-__host__ __device__ constexpr unsigned i8_idesc(int n) {
-    return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(I8_BM >> 4) << 24);
+// Arrives on `bar` when all products issued so far are done; with PAIR on the barriers at that place in both CTAs.
+template <bool PAIR>
+__device__ __forceinline__ void i8_commit(unsigned bar) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"((unsigned short)3)
+                     : "memory");
+    else
+        tc_commit(bar);
+}
+// int32 accumulator (2 at bit 4), signed operands (1 at bits 7 and 10), both K-major
+__host__ __device__ constexpr unsigned i8_idesc(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
 }
 
-// Eight (FP32) or eight (BF16) neighbouring outputs of a row.
+// 64 bytes of each of a warp's 32 rows, a lane's row in v, from output column `col` on.  Stored as they lie in the lanes a
+// request would touch 32 rows with half a sector each; through shared memory (16-byte pieces, exchanged by row so that eight
+// lanes use all banks) four lanes store a row's 64 bytes.
 template <bool F32>
-__device__ __forceinline__ void int8_store8(const Int8Params& p, long long row, int col, const float (&v)[8], bool vec) {
-    if constexpr (F32) {
-        float* y = reinterpret_cast<float*>(p.y) + row * p.y_stride + col;
-        if (vec && col + 8 <= p.outs) {
-            *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
+__device__ __forceinline__ void int8_store(const Int8Params& p, unsigned char* staging, int row0, int col, const float* v, bool vec) {
+    constexpr int PER = F32 ? 4 : 8, COLS = 4 * PER;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + e < p.outs) y[e] = v[e];
-        }
-    } else {
-        __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + row * p.y_stride + col;
-        if (vec && col + 8 <= p.outs) {
-            uint4 w;
+    for (int c = 0; c < 4; ++c) {
+        uint4 w;
+        if constexpr (F32) {
+            w = make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
+        } else {
             __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-            *reinterpret_cast<uint4*>(y) = w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + e < p.outs) y[e] = __float2bfloat16_rn(v[e]);
+            for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[8 * c + 2 * e], v[8 * c + 2 * e + 1]);
         }
+        *reinterpret_cast<uint4*>(staging + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16) = w;
+    }
+    __syncwarp();
+    using Out = typename std::conditional<F32, float, __nv_bfloat16>::type;
+    Out* y = reinterpret_cast<Out*>(p.y);
+    if (vec && col + COLS <= p.outs) {
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const int r = it * 8 + (lane >> 2), c = lane & 3;
+            const uint4 w = *reinterpret_cast<const uint4*>(staging + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
+            if (row0 + r < p.M) *reinterpret_cast<uint4*>(y + (row0 + r) * p.y_stride + col + c * PER) = w;
+        }
+        return;
+    }
+    // rows that start anywhere, or the last columns: an entry a lane
+    for (int idx = lane; idx < 32 * COLS; idx += 32) {
+        const int r = idx / COLS, e = idx % COLS;
+        if (row0 + r < p.M && col + e < p.outs)
+            y[(row0 + r) * p.y_stride + col + e] =
+                reinterpret_cast<const Out*>(staging + r * 64 + (((e / PER) ^ (r >> 1)) & 3) * 16)[e % PER];
     }
 }
 
-template <int BN, bool GATED, bool F32>
+template <int BN, bool GATED, bool F32, bool PAIR>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, int* fault) {
-    using Tile = Int8Tile<BN>;
-    constexpr int S = Tile::STAGES, OUTS = GATED ? BN / 2 : BN;
+    using Tile = Int8Tile<BN, PAIR>;
+    constexpr int S = Tile::STAGES, OUTS = GATED ? BN / 2 : BN, BM = PAIR ? 2 * I8_BM : I8_BM, CTAS = PAIR ? 2 : 1;
     extern __shared__ __align__(16) unsigned char i8_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * S + 4];   // full, empty, accumulator full, accumulator empty
     __shared__ unsigned s_tmem;
     __shared__ __align__(16) float s_scale[2][BN], s_bias[2][BN];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = PAIR ? blockIdx.x & 1 : 0;
     const unsigned ring = (tc_smem(i8_raw) + 1023u) & ~1023u;
+    unsigned char* const staging = i8_raw + (ring - tc_smem(i8_raw)) + S * Tile::STAGE_BYTES + (warp & 7) * I8_STAGING;
     const unsigned full0 = tc_smem(bars), empty0 = full0 + 8 * S, acc_full0 = empty0 + 8 * S, acc_empty0 = acc_full0 + 16;
+    const auto pair_barrier = [&]() {
+        if constexpr (PAIR) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        else __syncthreads();
+    };
 
     if (tid == 0) {
         for (int i = 0; i < 2 * S + 2; ++i)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8 * i));
         for (int i = 0; i < 2; ++i)
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty0 + 8 * i), "r"(I8_EPILOGUE_THREADS));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty0 + 8 * i), "r"(CTAS * I8_EPILOGUE_THREADS));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&s_tmem)), "r"(Tile::TMEM_COLS));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&s_tmem)), "r"(Tile::TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&s_tmem)), "r"(Tile::TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        }
     }
     tc_fence_before();
-    __syncthreads();
+    pair_barrier();
     tc_fence_after();
     chain_wait();   // the set-up above runs under the kernel that writes the rows
     chain_release();
     const unsigned tbase = s_tmem;
     const int tiles = p.tiles_m * p.tiles_n, blocks = (p.K + I8_BK - 1) / I8_BK;
+    const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
     // groups of I8_GROUP row tiles; inside one, the row tile changes first
     const auto place = [&](int tile, int& m, int& n) {
         const int per_group = I8_GROUP * p.tiles_n, g = tile / per_group, rest = tile - g * per_group;
@@ -248,36 +326,53 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
         n = rest / height;
         m = g * I8_GROUP + rest - n * height;
     };
+    // a barrier of the pair's first CTA
+    const auto of_first = [&](unsigned bar) {
+        unsigned a = bar;
+        if constexpr (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(bar));
+        return a;
+    };
 
     if (warp == 0) {   // ---- loads
         if (lane == 0) {
             int k = 0;   // stages filled so far
             bool alive = true;
-            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+            for (int tile = worker; tile < tiles && alive; tile += workers) {
                 int m, n;
                 place(tile, m, n);
-                for (int b = 0; b < blocks && alive; ++b, ++k) {
+                for (int b = 0; b < blocks; ++b, ++k) {
                     const int s = k % S;
                     if (k >= S) alive = tc_wait(empty0 + 8 * s, (k / S - 1) & 1);
                     if (!alive) break;
-                    const unsigned bar = full0 + 8 * s, a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(Tile::STAGE_BYTES) : "memory");
-                    tc_load_2d(a, &x_map, b * I8_BK, m * I8_BM, bar);
-                    tc_load_2d(w, &w_map, b * I8_BK, n * OUTS, bar);
-                    if (GATED) tc_load_2d(w + Tile::B_BYTES / 2, &w_map, b * I8_BK, p.outs + n * OUTS, bar);
+                    const unsigned bar = of_first(full0 + 8 * s), a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
+                    if (rank == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full0 + 8 * s),
+                                     "r"(CTAS * Tile::STAGE_BYTES)
+                                     : "memory");
+                    i8_load<PAIR>(a, &x_map, b * I8_BK, m * BM + rank * I8_BM, bar);
+                    if constexpr (PAIR) {   // the gate rows or the value rows; or either half
+                        i8_load<PAIR>(w, &w_map, b * I8_BK, GATED ? rank * p.outs + n * OUTS : n * OUTS + rank * Tile::B_ROWS, bar);
+                    } else {
+                        i8_load<PAIR>(w, &w_map, b * I8_BK, n * OUTS, bar);
+                        if (GATED) i8_load<PAIR>(w + Tile::B_BYTES / 2, &w_map, b * I8_BK, p.outs + n * OUTS, bar);
+                    }
                 }
             }
+            // with PAIR the first CTA's arrivals reach this one's memory: none is on its way when it leaves
+            for (int i = k > S ? k - S : 0; PAIR && i < k && alive; ++i) alive = tc_wait(empty0 + 8 * (i % S), (i / S) & 1);
             if (!alive) {
                 atomicExch(fault, 9);
-                for (int i = k > S ? k - S : 0; i < k; ++i) tc_wait(full0 + 8 * (i % S), (i / S) & 1);   // copies in flight
+                // copies in flight, into this CTA and (PAIR) the other, land before anyone leaves
+                if (rank == 0)
+                    for (int i = k > S ? k - S : 0; i < k; ++i) tc_wait(full0 + 8 * (i % S), (i / S) & 1);
             }
         }
         __syncwarp();
     } else if (warp == 1) {   // ---- products
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             int k = 0, t = 0;
             bool alive = true;
-            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x, ++t) {
+            for (int tile = worker; tile < tiles && alive; tile += workers, ++t) {
                 if (t >= 2) alive = tc_wait(acc_empty0 + 8 * (t & 1), (t / 2 - 1) & 1);
                 tc_fence_after();
                 const unsigned acc = tbase + (t & 1) * BN;
@@ -289,22 +384,21 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
                     const unsigned a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
 #pragma unroll
                     for (int j = 0; j < I8_BK / 32; ++j)
-                        i8_mma(acc, tc_desc(a + j * 32, 16, 1024) | (2ull << 61), tc_desc(w + j * 32, 16, 1024) | (2ull << 61),
-                               i8_idesc(BN), b > 0 || j > 0 ? 1u : 0u);
-                    tc_commit(empty0 + 8 * s);
+                        i8_mma<PAIR>(acc, tc_desc(a + j * 32, 16, 1024) | (2ull << 61), tc_desc(w + j * 32, 16, 1024) | (2ull << 61),
+                                     i8_idesc(BM, BN), b > 0 || j > 0 ? 1u : 0u);
+                    i8_commit<PAIR>(empty0 + 8 * s);
                 }
-                if (alive) tc_commit(acc_full0 + 8 * (t & 1));
+                if (alive) i8_commit<PAIR>(acc_full0 + 8 * (t & 1));
             }
             if (!alive) atomicExch(fault, 10);
         }
         __syncwarp();
     } else if (warp >= I8_EPILOGUE_WARP) {   // ---- scales, bias, gate, store
         const int quarter = warp & 3, half = (warp - I8_EPILOGUE_WARP) >> 2, etid = tid - I8_EPILOGUE_WARP * 32;
-        const int align = F32 ? 4 : 8;
-        const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.y_stride % align == 0;
+        const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.y_stride % (F32 ? 4 : 8) == 0;
         int t = 0;
         bool alive = true;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+        for (int tile = worker; tile < tiles; tile += workers, ++t) {
             int m, n;
             place(tile, m, n);
             float *scale = s_scale[t & 1], *bias = s_bias[t & 1];
@@ -315,8 +409,8 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
                 bias[etid] = col < p.outs ? int8_bias(p, w) : 0.f;
             }
             asm volatile("bar.sync 1, %0;" ::"n"(I8_EPILOGUE_THREADS) : "memory");
-            const int i = m * I8_BM + quarter * 32 + lane;
-            const float sx = i < p.M ? p.x_scale[i] : 0.f;
+            const int row0 = m * BM + rank * I8_BM + quarter * 32;
+            const float sx = row0 + lane < p.M ? p.x_scale[row0 + lane] : 0.f;
             if (alive) alive = tc_wait(acc_full0 + 8 * (t & 1), (t / 2) & 1);
             alive = __all_sync(0xffffffffu, alive);
             if (!alive) {
@@ -325,34 +419,35 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
             }
             tc_fence_after();
             const unsigned acc = tbase + (t & 1) * BN + ((unsigned)(quarter * 32) << 16);
-            constexpr int STEP = 16;
+            constexpr int STEP = F32 ? 16 : 32;   // 64 bytes of a row
 #pragma unroll 1
-            for (int c0 = half * (OUTS / 2); c0 < (half + 1) * (OUTS / 2); c0 += STEP) {
-                float r[STEP], g[STEP];
-                tc_ld16(acc + c0, r);
-                if (GATED) tc_ld16(acc + OUTS + c0, g);
+            for (int c0 = half * STEP; c0 < OUTS; c0 += 2 * STEP) {
+                if (row0 >= p.M || n * OUTS + c0 >= p.outs) break;
+                float v[STEP], g[GATED ? STEP : 1];
+                tc_ld<STEP>(acc + c0, v);
+                if constexpr (GATED) tc_ld<STEP>(acc + OUTS + c0, g);
                 tc_wait_ld();
 #pragma unroll
-                for (int e8 = 0; e8 < STEP; e8 += 8) {
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int c = c0 + e8 + e;
-                        v[e] = fmaf((float)__float_as_int(r[e8 + e]) * sx, scale[c], bias[c]);
-                        if (GATED)
-                            v[e] = int8_gated(v[e], fmaf((float)__float_as_int(g[e8 + e]) * sx, scale[OUTS + c], bias[OUTS + c]));
-                    }
-                    if (i < p.M && n * OUTS + c0 + e8 < p.outs) int8_store8<F32>(p, i, n * OUTS + c0 + e8, v, vec);
+                for (int e = 0; e < STEP; ++e) {
+                    const int c = c0 + e;
+                    v[e] = fmaf((float)__float_as_int(v[e]) * sx, scale[c], bias[c]);
+                    if constexpr (GATED) v[e] = int8_gated(v[e], fmaf((float)__float_as_int(g[e]) * sx, scale[OUTS + c], bias[OUTS + c]));
                 }
+                int8_store<F32>(p, staging, row0, n * OUTS + c0, v, vec);
             }
             tc_fence_before();
-            tc_arrive(acc_empty0 + 8 * (t & 1));
+            const unsigned bar = of_first(acc_empty0 + 8 * (t & 1));
+            asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
         }
     }
     tc_fence_before();
-    __syncthreads();
-    if (warp == 2)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(Tile::TMEM_COLS));
+    pair_barrier();   // with PAIR: nobody leaves while the other may arrive here, load here or read its operands here
+    if (warp == 2) {
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(Tile::TMEM_COLS));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(Tile::TMEM_COLS));
+    }
 }
 
 // ---- few rows: a cached token of a serving batch --------------------------------------------------------------------

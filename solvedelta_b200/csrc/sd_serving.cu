@@ -58,6 +58,20 @@ constexpr int MAX_K = 131072;   // 127 * 127 * K stays below 2^31
 int padded(int K) { return (K + 15) / 16 * 16; }
 
 // ---- quantised rows ----
+template <class T, bool VEC, int W, int H>
+int quantize_launch(const QuantizeParams& p, bool chained, cudaStream_t stream) {
+    return launch<k_quantize_rows<T, VEC, W, H>>((unsigned)((p.rows * W + 7) / 8), QUANT_THREADS, 0, 0, 1, chained, stream, p);
+}
+template <class T, bool VEC, int H>
+int quantize_width(const QuantizeParams& p, bool chained, cudaStream_t stream) {
+    // as few warps a row as hold it in registers, but more while the SMs are not full of warps (2048 rows: 32 each)
+    const auto enough = [&](int w) { return (long long)w * 256 * H >= p.K && p.rows * w >= 148 * 16; };
+    if (enough(1)) return quantize_launch<T, VEC, 1, H>(p, chained, stream);
+    if (enough(2)) return quantize_launch<T, VEC, 2, H>(p, chained, stream);
+    if (enough(4)) return quantize_launch<T, VEC, 4, H>(p, chained, stream);
+    if (p.K <= 8 * 256) return quantize_launch<T, VEC, 8, 1>(p, chained, stream);
+    return quantize_launch<T, VEC, 8, H>(p, chained, stream);
+}
 int quantize(const sd_quantize_rows_args* a, bool chained, cudaStream_t stream) {
     QuantizeParams p{};
     p.rows = a->rows; p.K = a->K;
@@ -65,12 +79,9 @@ int quantize(const sd_quantize_rows_args* a, bool chained, cudaStream_t stream) 
     p.q = reinterpret_cast<signed char*>(a->q); p.q_stride = a->q_stride;
     p.scale = a->scale;
     const bool f32 = a->x_type == SD_F32;
-    const bool vec = aligned(a->x) && a->x_stride % (f32 ? 4 : 8) == 0;
-    const unsigned rows = (unsigned)a->rows;
-    if (f32) return vec ? launch<k_quantize_rows<float, true>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p)
-                        : launch<k_quantize_rows<float, false>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p);
-    return vec ? launch<k_quantize_rows<__nv_bfloat16, true>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p)
-               : launch<k_quantize_rows<__nv_bfloat16, false>>(rows, QUANT_THREADS, 0, 0, 1, chained, stream, p);
+    const bool vec = aligned(a->x) && a->x_stride % (f32 ? 4 : 8) == 0 && a->K % 8 == 0;
+    if (f32) return vec ? quantize_width<float, true, 4>(p, chained, stream) : quantize_width<float, false, 4>(p, chained, stream);
+    return vec ? quantize_width<__nv_bfloat16, true, 8>(p, chained, stream) : quantize_width<__nv_bfloat16, false, 8>(p, chained, stream);
 }
 
 // ---- products ----
@@ -87,31 +98,32 @@ bool int8_map(CUtensorMap* map, const void* base, long long rows, int K, long lo
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool GATED, bool F32>
+template <int BN, bool GATED, bool F32, bool PAIR>
 int launch_matmul(Int8Params p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
-    constexpr int OUTS = GATED ? BN / 2 : BN;
+    constexpr int OUTS = GATED ? BN / 2 : BN, CTAS = PAIR ? 2 : 1;
     CUtensorMap x_map, w_map;
     int* fault = fault_word();
     if (fault == nullptr) return SD_ERR_NO_DEVICE;
-    if (!int8_map(&x_map, q, p.M, p.K, q_stride, I8_BM) || !int8_map(&w_map, a->weight, a->N, p.K, a->weight_stride, OUTS))
+    if (!int8_map(&x_map, q, p.M, p.K, q_stride, I8_BM) || !int8_map(&w_map, a->weight, a->N, p.K, a->weight_stride, PAIR || GATED ? BN / 2 : BN))
         return SD_ERR_LAUNCH_FAILED;
-    p.tiles_m = (p.M + I8_BM - 1) / I8_BM;
+    p.tiles_m = (p.M + CTAS * I8_BM - 1) / (CTAS * I8_BM);
     p.tiles_n = (p.outs + OUTS - 1) / OUTS;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     if (tiles > 0x7fffffffLL - 148) return SD_ERR_UNSUPPORTED_SHAPE;
-    return launch<k_int8_matmul<BN, GATED, F32>>((unsigned)(tiles < 148 ? tiles : 148), I8_THREADS, Int8Tile<BN>::SMEM,
-                                                 Int8Tile<BN>::SMEM, 1, chained, stream, p, x_map, w_map, fault);
+    const unsigned workers = (unsigned)(tiles < 148 / CTAS ? tiles : 148 / CTAS);
+    return launch<k_int8_matmul<BN, GATED, F32, PAIR>>(workers * CTAS, I8_THREADS, Int8Tile<BN, PAIR>::SMEM, Int8Tile<BN, PAIR>::SMEM, CTAS,
+                                                       chained, stream, p, x_map, w_map, fault);
 }
 template <bool GATED, bool F32>
 int matmul_tile(const Int8Params& p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
-    const auto tiles = [&](int bn) {
+    const auto tiles = [&](int bm, int bn) {
         const int outs = GATED ? bn / 2 : bn;
-        return (long long)((p.M + I8_BM - 1) / I8_BM) * ((p.outs + outs - 1) / outs);
+        return (long long)((p.M + bm - 1) / bm) * ((p.outs + outs - 1) / outs);
     };
     // the widest tile that still gives every SM one
-    if (tiles(256) >= 148) return launch_matmul<256, GATED, F32>(p, a, q, q_stride, chained, stream);
-    if (tiles(128) >= 148) return launch_matmul<128, GATED, F32>(p, a, q, q_stride, chained, stream);
-    return launch_matmul<64, GATED, F32>(p, a, q, q_stride, chained, stream);
+    if (tiles(256, 256) >= 74 && p.M > 128) return launch_matmul<256, GATED, F32, true>(p, a, q, q_stride, chained, stream);
+    if (tiles(128, 128) >= 148) return launch_matmul<128, GATED, F32, false>(p, a, q, q_stride, chained, stream);
+    return launch_matmul<64, GATED, F32, false>(p, a, q, q_stride, chained, stream);
 }
 int matmul(const Int8Params& p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
     if (a->swiglu) return p.out_f32 ? matmul_tile<true, true>(p, a, q, q_stride, chained, stream)
@@ -147,7 +159,7 @@ bool token_takes(const sd_int8_linear_args* a) { return a->rows <= I8_TOKEN_ROWS
 // Few entries: every CTA quantises the rows for itself, which saves a launch; past that its reading costs more.
 constexpr long long TOKEN_FUSED_ENTRIES = 16384;
 bool token_fuses(const sd_int8_linear_args* a) {
-    return token_takes(a) && a->x_type == SD_BF16 && aligned(a->x) && a->x_stride % 8 == 0 && a->rows * a->K <= TOKEN_FUSED_ENTRIES;
+    return token_takes(a) && a->x_type == SD_BF16 && aligned(a->x) && a->x_stride % 8 == 0 && a->K % 8 == 0 && a->rows * a->K <= TOKEN_FUSED_ENTRIES;
 }
 
 size_t q_bytes(const sd_int8_linear_args* a) { return ((size_t)a->rows * padded(a->K) + 255) / 256 * 256; }
