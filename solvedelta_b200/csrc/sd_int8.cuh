@@ -23,8 +23,6 @@ struct QuantizeParams {
     float* scale;
 };
 
-__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
 // What a row's largest magnitude (its bits) makes of the row.
 struct RowScale {
     float scale, inverse, largest;   // a / 127, about 127 / a, a
@@ -39,31 +37,18 @@ __device__ __forceinline__ RowScale row_scale(unsigned largest_bits) {
     r.inverse = r.special ? 0.f : __fdiv_rn(127.f, r.largest);
     return r;
 }
-// 127 x / a rounded to nearest even, where the product below leaves it open: 127 x is compared with half * a, both exact in
-// 64 bits.
-__device__ __noinline__ int quantize_exactly(float x, float inverse, float a) {
-    if (a < 1e-30f) return a == 0.f ? 0 : (int)rint(127.0 * (double)x / (double)a);
-    // the product is less than a half off, so the quotient lies between the neighbours of this half
-    const double low = floor((double)(x * inverse)), exact = 127.0 * (double)x, border = (low + 0.5) * (double)a;
-    return (int)(exact > border ? low + 1.0 : exact < border ? low : 2.0 * rint(low * 0.5 + 0.25));
+// 127 x / a rounded to nearest even.  The product with the rounded inverse is less than a half off, so the quotient lies between
+// the neighbours of the half h above its whole part; 127 x and h a, each with what FP32 rounds off, are compared exactly.  (BF16
+// rows come here often: the half of their largest entry is a tie.)
+__device__ __forceinline__ int quantize_exactly(float x, float inverse, float a) {
+    const float low = floorf(x * inverse), h = low + 0.5f, l = 127.f * x, r = h * a;
+    const float dl = fmaf(127.f, x, -l), dr = fmaf(h, a, -r);
+    const bool above = l > r || (l == r && dl > dr), tie = l == r && dl == dr;
+    const int n = (int)low;
+    return n + (above || (tie && (n & 1)) ? 1 : 0);
 }
-// Four entries as bytes.  x times the rounded inverse is at most 1.5 * 2^-23 of itself off, under 2^-15; its sum with
-// 1.5 * 2^23 is the nearest whole number, in the low bits, unless it lies that close to a half.
-__device__ __forceinline__ unsigned quantize_four(const float* v, const RowScale& r) {
-    unsigned w[4];
-    float far = 0.f;   // from the whole numbers
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float t = v[e] * r.inverse, n = t + 12582912.f;
-        far = fmaxf(far, fabsf(t - (n - 12582912.f)));
-        w[e] = __float_as_uint(n);
-    }
-    if (r.special || far > 0.5f - 3.1e-5f) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = r.bad ? 0u : (unsigned)quantize_exactly(v[e], r.inverse, r.largest);
-    }
-    return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
-}
+// The same for rows whose inverse may overflow.
+__device__ __noinline__ int quantize_tiny(float x, float a) { return a == 0.f ? 0 : (int)rint(127.0 * (double)x / (double)a); }
 
 template <class T>
 __device__ __forceinline__ float to_float(T v);
@@ -72,33 +57,83 @@ __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Eight entries of a row from column c0 on, zeros past its end.  VEC: rows start on 16-byte boundaries and K is a multiple of
-// eight, so that a request is one predicated instruction and a lane's requests go out together.
+// Eight entries of a row as they lie in memory.
+template <class T>
+struct Piece {
+    uint4 raw[sizeof(T) / 2];
+};
+// From column c0 on, zeros past the row's end.  VEC: rows start on 16-byte boundaries and K is a multiple of eight, so that a
+// request is one predicated instruction and a lane's requests go out together.
 template <class T, bool VEC>
-__device__ __forceinline__ void load_eight(const T* row, int c0, int K, float (&v)[8]) {
-    if constexpr (!VEC) {
+__device__ __forceinline__ Piece<T> load_piece(const T* row, int c0, int K) {
+    Piece<T> p;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c0 + e < K ? to_float(row[c0 + e]) : 0.f;
-    } else if constexpr (sizeof(T) == 2) {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (c0 < K) raw = *reinterpret_cast<const uint4*>(row + c0);
-        const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) p.raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (VEC) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = __bfloat1622float2(p[e]);
-            v[2 * e] = f.x;
-            v[2 * e + 1] = f.y;
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+            if (c0 < K) p.raw[i] = reinterpret_cast<const uint4*>(row + c0)[i];
+    } else {
+        T* e = reinterpret_cast<T*>(p.raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < K) e[i] = row[c0 + i];
+    }
+    return p;
+}
+// The larger of `top` and the entries' magnitudes, as FP32 bits but not yet reduced: piece_top() of BF16 keeps the even and the
+// odd entries' bits in two halves (infinities and NaNs are the largest numbers there as well).
+template <class T>
+__device__ __forceinline__ unsigned piece_top(const Piece<T>& p, unsigned top) {
+    const unsigned* w = reinterpret_cast<const unsigned*>(p.raw);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) * 2; ++i)
+        top = sizeof(T) == 2 ? __vmaxu2(top, w[i] & 0x7fff7fffu) : max(top, w[i] & 0x7fffffffu);
+    return top;
+}
+template <class T>
+__device__ __forceinline__ unsigned whole_top(unsigned top) { return sizeof(T) == 2 ? max(top & 0xffff0000u, top << 16) : top; }
+
+// The entries as bytes.  With b = 384.5 + 2^-15 the sum 127 x / a + b has eight bits of q + 128 and 15 bits behind the point; the
+// product with the rounded inverse and the sum are off by less than 2^-15 together (1.5 * 2^-23 of 127, and half a unit), so q is
+// right unless those 15 bits are 0, 1 or 2, next to where it changes.
+template <class T>
+__device__ __forceinline__ uint2 quantize_piece(const Piece<T>& p, const RowScale& r) {
+    float v[8];
+    unsigned u[8], near = 0xffffffffu;
+    if constexpr (sizeof(T) == 2) {
+        const unsigned* w = reinterpret_cast<const unsigned*>(p.raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     } else {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (c0 < K) {
-            a = *reinterpret_cast<const float4*>(row + c0);
-            b = *reinterpret_cast<const float4*>(row + c0 + 4);
-        }
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        const float* f = reinterpret_cast<const float*>(p.raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = f[i];
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        u[i] = __float_as_uint(fmaf(v[i], r.inverse, 384.5f + 0x1p-15f));
+        near = min(near, u[i] & 0x7fffu);
+        u[i] <<= 1;   // q + 128 in the third byte
+    }
+    if (near <= 2 || r.special) {
+        if (!r.special) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = (unsigned)(quantize_exactly(v[i], r.inverse, r.largest) + 128) << 16;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = (unsigned)((r.bad ? 0 : quantize_tiny(v[i], r.largest)) + 128) << 16;
+        }
+    }
+    uint2 out;
+    out.x = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410) ^ 0x80808080u;
+    out.y = __byte_perm(__byte_perm(u[4], u[5], 0x0062), __byte_perm(u[6], u[7], 0x0062), 0x5410) ^ 0x80808080u;
+    return out;
 }
+
 // Groups of W warps take a row each, eight rows to W = 1 in a CTA; a lane keeps up to H pieces of eight entries between the
 // search for the largest magnitude and the rounding (longer rows are read again).  q rows start on 16-byte boundaries,
 // q_stride covers K rounded up to 16, and the bytes past K are set to zero.
@@ -112,20 +147,14 @@ __global__ void __launch_bounds__(QUANT_THREADS) k_quantize_rows(QuantizeParams 
     const long long r_idx = (long long)blockIdx.x * (8 / W) + warp / W;
     const bool live = r_idx < p.rows;   // the rows of a CTA share its barrier
     const T* row = reinterpret_cast<const T*>(p.x) + (live ? r_idx : 0) * p.x_stride;
-    float held[H][8];
+    Piece<T> held[H];
     unsigned top = 0;
 #pragma unroll
-    for (int h = 0; h < H; ++h) load_eight<T, VEC>(row, (h * W * 32 + at) * 8, p.K, held[h]);
+    for (int h = 0; h < H; ++h) held[h] = load_piece<T, VEC>(row, (h * W * 32 + at) * 8, p.K);
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, abs_bits(held[h][e]));
-    for (int c0 = (H * W * 32 + at) * 8; c0 < p.K; c0 += W * 256) {
-        float v[8];
-        load_eight<T, VEC>(row, c0, p.K, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
-    }
+    for (int h = 0; h < H; ++h) top = piece_top(held[h], top);
+    for (int c0 = (H * W * 32 + at) * 8; c0 < p.K; c0 += W * 256) top = piece_top(load_piece<T, VEC>(row, c0, p.K), top);
+    top = whole_top<T>(top);
     top = __reduce_max_sync(0xffffffffu, top);
     if constexpr (W > 1) {
         if ((threadIdx.x & 31) == 0) s_max[warp] = top;
@@ -139,13 +168,10 @@ __global__ void __launch_bounds__(QUANT_THREADS) k_quantize_rows(QuantizeParams 
 #pragma unroll
     for (int h = 0; h < H; ++h) {
         const int c0 = (h * W * 32 + at) * 8;
-        if (c0 < padded) *reinterpret_cast<uint2*>(out + c0) = make_uint2(quantize_four(held[h], r), quantize_four(held[h] + 4, r));
+        if (c0 < padded) *reinterpret_cast<uint2*>(out + c0) = quantize_piece(held[h], r);
     }
-    for (int c0 = (H * W * 32 + at) * 8; c0 < padded; c0 += W * 256) {
-        float v[8];
-        load_eight<T, VEC>(row, c0, p.K, v);
-        *reinterpret_cast<uint2*>(out + c0) = make_uint2(quantize_four(v, r), quantize_four(v + 4, r));
-    }
+    for (int c0 = (H * W * 32 + at) * 8; c0 < padded; c0 += W * 256)
+        *reinterpret_cast<uint2*>(out + c0) = quantize_piece(load_piece<T, VEC>(row, c0, p.K), r);
     if (at == 0) p.scale[r_idx] = r.scale;
 }
 
@@ -480,7 +506,7 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, un
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // A 16-byte piece of a weight row: read once by one CTA, and ahead of the wait for the kernel before.
-__device__ __forceinline__ uint4 load_piece(const signed char* p) {
+__device__ __forceinline__ uint4 load_weight(const signed char* p) {
     uint4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
@@ -514,21 +540,16 @@ __device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char*
         __syncthreads();
         for (int u = warp; u < M * segs; u += 8) {
             const int m = u / segs, c0 = (u - m * segs) * 256 + lane * 8;
-            float v[8];
-            load_eight<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K, v);
-            unsigned top = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
-            top = __reduce_max_sync(0xffffffffu, top);
+            const Piece<T> piece = load_piece<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K);
+            const unsigned top = __reduce_max_sync(0xffffffffu, whole_top<T>(piece_top(piece, 0)));
             if (lane == 0) atomicMax(s_top + m, top);
         }
         __syncthreads();
         for (int u = warp; u < M * segs; u += 8) {
             const int m = u / segs, c0 = (u - m * segs) * 256 + lane * 8;
             const RowScale r = row_scale(s_top[m]);
-            float v[8];
-            load_eight<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K, v);
-            if (c0 < pitch) *reinterpret_cast<uint2*>(s_q + (long long)m * pitch + c0) = make_uint2(quantize_four(v, r), quantize_four(v + 4, r));
+            const Piece<T> piece = load_piece<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K);
+            if (c0 < pitch) *reinterpret_cast<uint2*>(s_q + (long long)m * pitch + c0) = quantize_piece(piece, r);
             if (c0 == 0) s_scale[m] = r.scale;
         }
     }
@@ -563,7 +584,7 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             const int c = base + i;
-            w[i] = ok && c < end && c * 64 + t * 16 < K ? load_piece(row + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+            w[i] = ok && c < end && c * 64 + t * 16 < K ? load_weight(row + c * 64) : make_uint4(0u, 0u, 0u, 0u);
         }
     };
     uint4 wa[B], wb[B];
