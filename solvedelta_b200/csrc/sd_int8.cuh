@@ -337,6 +337,8 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
         }
     }
+    if (warp == 3 && lane < 2)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(lane == 0 ? &x_map : &w_map)) : "memory");
     tc_fence_before();
     pair_barrier();
     tc_fence_after();
@@ -453,11 +455,22 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
                 tc_ld<STEP>(acc + c0, v);
                 if constexpr (GATED) tc_ld<STEP>(acc + OUTS + c0, g);
                 tc_wait_ld();
+                // (shared memory is what the products are short of: without a bias none is read)
 #pragma unroll
                 for (int e = 0; e < STEP; ++e) {
-                    const int c = c0 + e;
-                    v[e] = fmaf((float)__float_as_int(v[e]) * sx, scale[c], bias[c]);
-                    if constexpr (GATED) v[e] = int8_gated(v[e], fmaf((float)__float_as_int(g[e]) * sx, scale[OUTS + c], bias[OUTS + c]));
+                    v[e] = (float)__float_as_int(v[e]) * sx * scale[c0 + e];
+                    if constexpr (GATED) g[e] = (float)__float_as_int(g[e]) * sx * scale[OUTS + c0 + e];
+                }
+                if (p.bias != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < STEP; ++e) {
+                        v[e] += bias[c0 + e];
+                        if constexpr (GATED) g[e] += bias[OUTS + c0 + e];
+                    }
+                }
+                if constexpr (GATED) {
+#pragma unroll
+                    for (int e = 0; e < STEP; ++e) v[e] = int8_gated(v[e], g[e]);
                 }
                 int8_store<F32>(p, staging, row0, n * OUTS + c0, v, vec);
             }
@@ -518,40 +531,46 @@ __device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char*
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, M = p.o.M, K = p.o.K;
     const int pitch = (int)int8_pitch(K);
     if constexpr (sizeof(T) == 1) {
-        const int pieces = pitch / 16;
+        const int pieces = pitch / 16;   // asynchronous copies: all rows in flight at once, what lies past K comes as zeros
         for (int idx = tid; idx < M * pieces; idx += 256) {
-            const int m = idx / pieces, c0 = (idx - m * pieces) * 16;
-            const signed char* row = reinterpret_cast<const signed char*>(p.x) + m * p.x_stride;
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if (VEC && c0 + 16 <= K) {
-                w = *reinterpret_cast<const uint4*>(row + c0);
-            } else {
-                unsigned* u = reinterpret_cast<unsigned*>(&w);
-                for (int e = 0; e < 16; ++e)
-                    if (c0 + e < K) u[e / 4] |= (unsigned)(row[c0 + e] & 0xff) << (8 * (e % 4));
-            }
-            *reinterpret_cast<uint4*>(s_q + (long long)m * pitch + c0) = w;
+            const int m = idx / pieces, c0 = (idx - m * pieces) * 16, n = min(16, max(0, K - c0));
+            const signed char* from = reinterpret_cast<const signed char*>(p.x) + m * p.x_stride + (n > 0 ? c0 : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc_smem(s_q + (long long)m * pitch + c0)), "l"(from), "r"(n) : "memory");
         }
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         if (tid < M) s_scale[tid] = p.o.x_scale[tid];
     } else {
-        // units of 256 entries of a row, a warp each
-        const int segs = (pitch + 255) / 256;
-        if (tid < M) s_top[tid] = 0;
-        __syncthreads();
-        for (int u = warp; u < M * segs; u += 8) {
-            const int m = u / segs, c0 = (u - m * segs) * 256 + lane * 8;
-            const Piece<T> piece = load_piece<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K);
+        // units of 256 entries of a row, a warp each; the first HELD of a warp stay in registers between the two passes
+        constexpr int HELD = 4;
+        const int segs = (pitch + 255) / 256, units = M * segs;
+        const auto unit = [&](int u) {
+            const int m = u / segs;
+            return load_piece<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, u < units ? (u - m * segs) * 256 + lane * 8 : K, K);
+        };
+        const auto widen = [&](int u, const Piece<T>& piece) {
+            if (u >= units) return;
             const unsigned top = __reduce_max_sync(0xffffffffu, whole_top<T>(piece_top(piece, 0)));
-            if (lane == 0) atomicMax(s_top + m, top);
-        }
-        __syncthreads();
-        for (int u = warp; u < M * segs; u += 8) {
+            if (lane == 0) atomicMax(s_top + u / segs, top);
+        };
+        const auto store = [&](int u, const Piece<T>& piece) {
+            if (u >= units) return;
             const int m = u / segs, c0 = (u - m * segs) * 256 + lane * 8;
             const RowScale r = row_scale(s_top[m]);
-            const Piece<T> piece = load_piece<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, c0, K);
             if (c0 < pitch) *reinterpret_cast<uint2*>(s_q + (long long)m * pitch + c0) = quantize_piece(piece, r);
             if (c0 == 0) s_scale[m] = r.scale;
-        }
+        };
+        Piece<T> held[HELD];
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) held[h] = unit(warp + 8 * h);
+        if (tid < M) s_top[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) widen(warp + 8 * h, held[h]);
+        for (int u = warp + 8 * HELD; u < units; u += 8) widen(u, unit(u));
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) store(warp + 8 * h, held[h]);
+        for (int u = warp + 8 * HELD; u < units; u += 8) store(u, unit(u));
     }
 }
 
@@ -595,10 +614,22 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
     int8_rows<T, VEC>(p, s_q, s_scale, s_top);
     __syncthreads();
 
+    // the columns that a thread finishes are the same ones of every tile
+    const int out_col = tid % WIDTH;
+    float scale[2], bias[2];
+    const auto finish_of = [&](int tile) {
+        const int n = tile * WIDTH + out_col;
+#pragma unroll
+        for (int j = 0; j < (GATED ? 2 : 1); ++j) {
+            scale[j] = n < outs ? p.o.w_scale[n + j * outs] : 0.f;
+            bias[j] = n < outs ? int8_bias(p.o, n + j * outs) : 0.f;
+        }
+    };
     int acc[MT][4];
     const auto step = [&](int item, uint4 (&w)[B]) {
         const int st = item % steps, base = begin + st * B;
         if (st == 0) {
+            finish_of(blockIdx.x + item / steps * gridDim.x);   // requested ahead of the products
 #pragma unroll
             for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -632,18 +663,16 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
             }
         }
         __syncthreads();
-        const int n0 = (blockIdx.x + tile_no * gridDim.x) * WIDTH;
-        for (int idx = tid; idx < M * WIDTH; idx += 256) {
-            const int m = idx / WIDTH, c = idx - m * WIDTH, n = n0 + c;
-            if (n >= outs) continue;
-            const auto value = [&](int group, int w_row) {
+        const int n = (blockIdx.x + tile_no * gridDim.x) * WIDTH + out_col;
+        for (int m = tid / WIDTH; m < M && n < outs; m += 256 / WIDTH) {
+            const auto value = [&](int group, int j) {
                 int v = 0;
 #pragma unroll
-                for (int k = 0; k < KS; ++k) v += s_red[buf][k * CG + group][m][c & 7];
-                return fmaf((float)v * s_scale[m], p.o.w_scale[w_row], int8_bias(p.o, w_row));
+                for (int k = 0; k < KS; ++k) v += s_red[buf][k * CG + group][m][out_col & 7];
+                return (float)v * s_scale[m] * scale[j] + bias[j];
             };
-            float out = value(GATED ? 0 : c >> 3, n);
-            if (GATED) out = int8_gated(out, value(1, n + outs));
+            float out = value(GATED ? 0 : out_col >> 3, 0);
+            if constexpr (GATED) out = int8_gated(out, value(1, 1));
             if (p.o.out_f32) reinterpret_cast<float*>(p.o.y)[m * p.o.y_stride + n] = out;
             else reinterpret_cast<__nv_bfloat16*>(p.o.y)[m * p.o.y_stride + n] = __float2bfloat16_rn(out);
         }
