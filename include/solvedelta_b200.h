@@ -550,6 +550,8 @@ typedef struct {
     int64_t y_stride;
     void *scratch;
     size_t scratch_bytes;
+    int32_t chained;               /* the first launch may start under the kernel before it in the stream: that kernel must not
+                                    * write the weight, and must itself run behind whatever did */
 } sd_int8_linear_args;
 
 int sd_quantize_rows(const sd_quantize_rows_args *args, void *stream);

@@ -8,7 +8,7 @@ sm_100a CUDA kernels behind a C ABI (include/solvedelta_b200.h).
 """
 from ._lib import build, load
 from .config import SolveDeltaConfig
-from .int8_ops import int8_linear, int8_matmul, quantize_rows
+from .int8_ops import Int8Linear, int8_gated_mlp, int8_linear, int8_matmul, quantize_rows
 from .mixer_ops import conv4_silu, conv4_silu_segmented, kda_decay_gate, rms_norm_gated, rms_norm_gated_linear
 from .model import RMSNormGated, SolveDelta, SolveDeltaLayerState
 from .modeling import (GraphedDecoder, SolveDeltaBlock, SolveDeltaCache, SolveDeltaCacheAdapter, SolveDeltaForCausalLM,
@@ -73,6 +73,8 @@ __all__ = [
     "pack_tokens",
     "unpack_tokens",
     "solvedelta_zero_state",
+    "Int8Linear",
+    "int8_gated_mlp",
     "int8_linear",
     "int8_matmul",
     "quantize_rows",

@@ -290,7 +290,7 @@ class Int8LinearArgs(ctypes.Structure):
                 ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("x_scale", ctypes.c_void_p),
                 ("weight", ctypes.c_void_p), ("weight_stride", ctypes.c_int64), ("weight_scale", ctypes.c_void_p),
                 ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64),
-                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t)]
+                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t), ("chained", ctypes.c_int32)]
 
 
 class SampleTokensArgs(ctypes.Structure):

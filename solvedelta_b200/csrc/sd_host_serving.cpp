@@ -70,9 +70,17 @@ py::tuple quantize_rows(const Tensor& x) {
     return py::make_tuple(q, scale.view(shape));
 }
 
-// x: BF16 / FP32 rows, or int8 rows with their scales
+at::ScalarType output_type(const py::object& dtype) {
+    type_error(!THPDtype_Check(dtype.ptr()), "out_dtype must be torch.bfloat16 or torch.float32");
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+    type_error(type != at::kBFloat16 && type != at::kFloat, "out_dtype must be torch.bfloat16 or torch.float32");
+    return type;
+}
+
+// x: BF16 / FP32 rows, or int8 rows with their scales.  `chained`: the kernel before is this library's, launched behind
+// everything that may have written the weight.
 Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in, const Tensor& weight_scale_in,
-               const OptTensor& bias_in, bool swiglu, const py::object& out_dtype) {
+               const OptTensor& bias_in, bool swiglu, at::ScalarType out_type, bool chained = false) {
     const Tensor bias = given(bias_in);
     const bool quantized = scale_in.defined();
     type_error(!weight_in.is_cuda() || weight_in.scalar_type() != at::kChar, "weight must be an int8 CUDA tensor");
@@ -87,13 +95,6 @@ Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in,
     if (bias.defined()) {
         type_error(!is_real(bias), "bias must be BF16 or FP32");
         value_error(!is_shape(bias, {N}), "bias must be [N]");
-    }
-    at::ScalarType out_type;
-    {
-        const auto* dtype = reinterpret_cast<THPDtype*>(out_dtype.ptr());
-        type_error(!THPDtype_Check(out_dtype.ptr()), "out_dtype must be torch.bfloat16 or torch.float32");
-        out_type = dtype->scalar_type;
-        type_error(out_type != at::kBFloat16 && out_type != at::kFloat, "out_dtype must be torch.bfloat16 or torch.float32");
     }
     for (const Tensor* t : {&weight_in, &weight_scale_in, &bias, &scale_in})
         value_error(t->defined() && t->device() != x.device(), "all tensors must be on the device of the rows");
@@ -115,6 +116,9 @@ Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in,
     const Tensor weight = readable(weight_in.detach()), weight_scale = weight_scale_in.detach().contiguous();
     const Tensor scale = quantized ? scale_in.detach().reshape({M}).contiguous() : Tensor();
     const Tensor b = bias.defined() ? bias.detach().contiguous() : Tensor();
+    // a copy made here is written by the kernel before
+    chained = chained && weight.data_ptr() == weight_in.data_ptr() && weight_scale.data_ptr() == weight_scale_in.data_ptr() &&
+              (!b.defined() || b.data_ptr() == bias.data_ptr());
     sd_int8_linear_args a{};
     a.rows = M; a.N = (int32_t)N; a.K = (int32_t)K; a.swiglu = swiglu ? 1 : 0;
     a.x_type = quantized ? SD_I8 : element_type(rows); a.y_type = out_type == at::kFloat ? SD_F32 : SD_BF16;
@@ -124,7 +128,7 @@ Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in,
     a.y = y.data_ptr(); a.y_stride = shape.back();
     const size_t need = sd_int8_linear_scratch_bytes(&a);
     const Tensor scratch = need > 0 ? workspace(x, need) : Tensor();
-    a.scratch = raw(scratch); a.scratch_bytes = need;
+    a.scratch = raw(scratch); a.scratch_bytes = need; a.chained = chained ? 1 : 0;
     check(sd_int8_linear(&a, stream_of(x)));
     return y;
 }
@@ -132,12 +136,20 @@ Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in,
 Tensor int8_linear(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const OptTensor& bias, bool swiglu,
                    const py::object& out_dtype) {
     type_error(!x.is_cuda() || !is_real(x), "x must be a BF16 or FP32 CUDA tensor");
-    return product(x, Tensor(), weight, weight_scale, bias, swiglu, out_dtype);
+    return product(x, Tensor(), weight, weight_scale, bias, swiglu, output_type(out_dtype));
 }
 Tensor int8_matmul(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const OptTensor& bias,
                    bool swiglu, const py::object& out_dtype) {
     type_error(!q.is_cuda() || q.scalar_type() != at::kChar, "q must be an int8 CUDA tensor");
-    return product(q, scale, weight, weight_scale, bias, swiglu, out_dtype);
+    return product(q, scale, weight, weight_scale, bias, swiglu, output_type(out_dtype));
+}
+
+// The gated MLP: its second product is chained to the first.
+Tensor int8_gated_mlp(const Tensor& x, const Tensor& up, const Tensor& up_scale, const OptTensor& up_bias, const Tensor& down,
+                      const Tensor& down_scale, const OptTensor& down_bias) {
+    type_error(!x.is_cuda() || !is_real(x), "x must be a BF16 or FP32 CUDA tensor");
+    const Tensor act = product(x, Tensor(), up, up_scale, up_bias, true, at::kBFloat16);
+    return product(act, Tensor(), down, down_scale, down_bias, false, at::kBFloat16, true);
 }
 
 // ---- sampling -----------------------------------------------------------------------------------------------
@@ -193,5 +205,6 @@ void register_serving(py::module_& m) {
     m.def("quantize_rows", &quantize_rows);
     m.def("int8_linear", &int8_linear);
     m.def("int8_matmul", &int8_matmul);
+    m.def("int8_gated_mlp", &int8_gated_mlp);
     m.def("sample_tokens", &sample_tokens);
 }

@@ -228,11 +228,12 @@ int sd_int8_linear(const sd_int8_linear_args* a, void* stream_) {
     p.bias = a->bias; p.bias_f32 = a->bias_type == SD_F32;
     p.y = a->y; p.y_stride = a->y_stride; p.out_f32 = a->y_type == SD_F32;
     const bool token = token_takes(a);
+    bool chained = a->chained != 0;
     Int8TokenParams t{};
     t.W = reinterpret_cast<const signed char*>(a->weight); t.w_stride = a->weight_stride;
     if (token_fuses(a)) {
         t.o = p; t.x = a->x; t.x_stride = a->x_stride;
-        return token_rows<__nv_bfloat16, true>(t, a->swiglu != 0, false, stream);
+        return token_rows<__nv_bfloat16, true>(t, a->swiglu != 0, chained, stream);
     }
     const void* q = a->x;
     long long q_stride = a->x_stride;
@@ -243,15 +244,16 @@ int sd_int8_linear(const sd_int8_linear_args* a, void* stream_) {
         r.rows = a->rows; r.K = a->K; r.x_type = a->x_type; r.x = a->x; r.x_stride = a->x_stride;
         r.q = a->scratch; r.q_stride = padded(a->K);
         r.scale = reinterpret_cast<float*>(reinterpret_cast<char*>(a->scratch) + q_bytes(a));
-        const int e = quantize(&r, false, stream);
+        const int e = quantize(&r, chained, stream);
         if (e != SD_OK) return e;
         q = r.q; q_stride = r.q_stride; p.x_scale = r.scale;
+        chained = true;
     }
     if (token) {
         t.o = p; t.x = q; t.x_stride = q_stride;
-        return token_rows<signed char, true>(t, a->swiglu != 0, !quantized, stream);
+        return token_rows<signed char, true>(t, a->swiglu != 0, chained, stream);
     }
-    return matmul(p, a, q, q_stride, !quantized, stream);
+    return matmul(p, a, q, q_stride, chained, stream);
 }
 
 int sd_sample_tokens(const sd_sample_tokens_args* a, void* stream_) {

@@ -39,4 +39,61 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     return _lib.host().int8_linear(x, weight, weight_scale, bias, swiglu, out_dtype)
 
 
-__all__ = ["int8_linear", "int8_matmul", "quantize_rows"]
+def int8_gated_mlp(x: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor, up_bias: Optional[torch.Tensor],
+                   down: torch.Tensor, down_scale: torch.Tensor, down_bias: Optional[torch.Tensor]) -> torch.Tensor:
+    """``int8_linear(int8_linear(x, up, up_scale, up_bias, swiglu=True), down, down_scale, down_bias)`` in one native call,
+    the 8-bit counterpart of :func:`mixer_ops.gated_mlp`: ``up`` holds gate rows and as many value rows; BF16 out."""
+    return _lib.host().int8_gated_mlp(x, up, up_scale, up_bias, down, down_scale, down_bias)
+
+
+class Int8Linear(nn.Module):
+    """A projection for inference whose weight is held in int8 with a scale for each output channel (buffers ``weight``
+    ``[out, in]``, ``weight_scale`` ``[out]`` and, where there is one, ``bias``); the rows it is given are quantised row by
+    row on the way in.  Not trainable: with gradients recorded for its input it raises."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, device=None) -> None:
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        # rows start on 16-byte boundaries, as the kernels read them
+        pitch = (in_features + 15) // 16 * 16
+        weight = torch.zeros(out_features, pitch, dtype=torch.int8, device=device)[:, :in_features]
+        self.register_buffer("weight", weight)
+        self.register_buffer("weight_scale", torch.zeros(out_features, dtype=torch.float32, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.bfloat16, device=device) if bias else None)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
+        """The projection of a CUDA ``nn.Linear`` (BF16 or FP32), its weight quantised output channel by output channel."""
+        weight = linear.weight.detach()
+        made = cls(linear.in_features, linear.out_features, linear.bias is not None, weight.device)
+        q, scale = quantize_rows(weight)
+        if not torch.isfinite(scale).all():
+            raise ValueError("a weight with infinities or NaNs cannot be quantised")
+        made.weight.copy_(q)
+        made.weight_scale.copy_(scale)
+        if linear.bias is not None:
+            made.bias.copy_(linear.bias.detach())
+        return made.train(linear.training)
+
+    def _apply(self, fn, recurse: bool = True):
+        # a change of the module's floating type (model.bfloat16(), model.half()) is not one of the scales
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        if self.weight.stride(0) % 16 != 0:   # moved without its padding
+            pitch = (self.in_features + 15) // 16 * 16
+            padded = torch.zeros(self.out_features, pitch, dtype=torch.int8, device=self.weight.device)
+            self.weight = padded[:, :self.in_features].copy_(self.weight)
+        if self.bias is not None and self.bias.dtype not in (torch.bfloat16, torch.float32):
+            self.bias = self.bias.to(torch.bfloat16)
+        return self
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int8_linear(x, self.weight, self.weight_scale, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+__all__ = ["Int8Linear", "int8_gated_mlp", "int8_linear", "int8_matmul", "quantize_rows"]

@@ -24,9 +24,11 @@ from transformers.modeling_outputs import BaseModelOutputWithPast, CausalLMOutpu
 
 from . import _lib
 from .config import SolveDeltaConfig
+from .int8_ops import Int8Linear, int8_gated_mlp
 from .ops import SolveDeltaState
 from .mixer_ops import add_rmsnorm, add_rmsnorm_reverse_supported, gated_mlp, swiglu
 from .model import SolveDelta, SolveDeltaLayerState
+from .sampling import sample_tokens
 from .token_stack import token_stack
 
 FP32_PARAMETERS = ("geometry_write_bias", "associative_log_rate", "associative_decay_bias")
@@ -108,10 +110,10 @@ def segment_reset_mask(hidden_states: torch.Tensor, cu_seqlens: torch.Tensor) ->
     return mask.unsqueeze(0)
 
 
-def _bare_linear(layer: nn.Module) -> bool:
-    """A plain ``nn.Linear`` whose call does nothing beside its product: no hook, adapter, parametrisation or replaced
-    ``forward``, so that its weight may be used in its place."""
-    return (type(layer) is nn.Linear and "forward" not in layer.__dict__
+def _bare_linear(layer: nn.Module, kind: type = nn.Linear) -> bool:
+    """A plain ``nn.Linear`` (or ``kind``) whose call does nothing beside its product: no hook, adapter, parametrisation or
+    replaced ``forward``, so that its weight may be used in its place."""
+    return (type(layer) is kind and "forward" not in layer.__dict__
             and not (layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks
                      or layer._backward_pre_hooks or module_globals._has_any_global_hook()))
 
@@ -143,6 +145,8 @@ class SolveDeltaMLP(nn.Module):
         kernels = self.hidden_act == "swish" and x.is_cuda and x.dtype == torch.bfloat16
         if kernels and _bare_linear(up) and _bare_linear(down):
             return gated_mlp(x, up.weight, up.bias, down.weight, down.bias)
+        if kernels and _bare_linear(up, Int8Linear) and _bare_linear(down, Int8Linear):
+            return int8_gated_mlp(x, up.weight, up.weight_scale, up.bias, down.weight, down.weight_scale, down.bias)
         gate_value = up(x)
         if kernels and gate_value.dtype == torch.bfloat16:
             return down(swiglu(gate_value))   # activation and product in one kernel
@@ -430,6 +434,20 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
             parameter.data = parameter.data.to(torch.float32 if keep else torch.bfloat16)
         return self
 
+    def quantize_int8(self, head: bool = False) -> "SolveDeltaForCausalLM":
+        """Hold the gated MLPs' weights, and with ``head`` the vocabulary projection's, in int8 (:class:`Int8Linear`), for
+        inference on a CUDA device: half of their bytes in a cached token, twice the tensor rate in a prompt.  The mixers
+        stay in BF16.  In place, not reversible; quantised modules are left as they are.  Returns the model."""
+        if head and self.config.tie_word_embeddings:
+            raise ValueError("a tied head shares the embedding's weight and cannot be quantised")
+        for layer in self.model.layers:
+            for name in ("gate_up_proj", "down_proj"):
+                if not isinstance(getattr(layer.mlp, name), Int8Linear):
+                    setattr(layer.mlp, name, Int8Linear.from_linear(getattr(layer.mlp, name)))
+        if head and not isinstance(self.lm_head, Int8Linear):
+            self.lm_head = Int8Linear.from_linear(self.lm_head)
+        return self
+
     def _plain_head(self) -> bool:
         """The head is a bare projection and nothing is hooked to it or to the inner model."""
         head, inner = self.lm_head, self.model
@@ -503,16 +521,14 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
         return CausalLMOutputWithPast(loss=loss, logits=logits, past_key_values=outputs.past_key_values,
                                       hidden_states=outputs.hidden_states)
 
-    @torch.no_grad()
-    def greedy_generate(self, input_ids: torch.Tensor, max_new_tokens: int, graphed: bool = False) -> torch.Tensor:
-        """Greedy decoding through the cache: one prefill, then one-token steps (replayed from a
-        CUDA graph when ``graphed``)."""
+    def _generate(self, input_ids: torch.Tensor, max_new_tokens: int, graphed: bool, choose) -> torch.Tensor:
+        """One prefill, then one-token steps through the cache; ``choose(logits [B, vocab], step)`` gives the tokens [B]."""
         step = self(input_ids=input_ids, use_cache=True, logits_to_keep=1)
         cache, tokens = step.past_key_values, [input_ids]
         logits = step.logits
         decoder = GraphedDecoder(self, cache, input_ids.shape[0]) if graphed and max_new_tokens > 0 else None
-        for _ in range(max_new_tokens):
-            nxt = logits[:, -1].argmax(dim=-1, keepdim=True)
+        for n in range(max_new_tokens):
+            nxt = choose(logits[:, -1], n).unsqueeze(1)
             tokens.append(nxt)
             if decoder is not None:
                 logits = decoder.step(nxt)
@@ -520,6 +536,30 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
                 logits = self(input_ids=nxt, past_key_values=cache, use_cache=True, logits_to_keep=1).logits
         _lib.check_device_fault()   # one synchronisation at the end of the loop: every bounded wait completed
         return torch.cat(tokens, dim=1)
+
+    @torch.no_grad()
+    def greedy_generate(self, input_ids: torch.Tensor, max_new_tokens: int, graphed: bool = False) -> torch.Tensor:
+        """Greedy decoding through the cache: one prefill, then one-token steps (replayed from a
+        CUDA graph when ``graphed``)."""
+        return self._generate(input_ids, max_new_tokens, graphed, lambda logits, n: logits.argmax(dim=-1))
+
+    @torch.no_grad()
+    def sample_generate(self, input_ids: torch.Tensor, max_new_tokens: int, *,
+                        temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
+                        top_p: Union[float, torch.Tensor] = 1.0, min_p: Union[float, torch.Tensor] = 0.0,
+                        uniform: Optional[torch.Tensor] = None, generator: Optional[torch.Generator] = None,
+                        graphed: bool = False) -> torch.Tensor:
+        """:meth:`greedy_generate` with tokens drawn by :func:`sample_tokens`: every setting a number or a tensor ``[B]``
+        (a row of temperature 0 is greedy).  The draws come from ``uniform``, FP32 ``[max_new_tokens, B]`` in [0, 1), or
+        from ``generator``.  A row without a finite logit continues with the padding token, or token 0."""
+        batch = input_ids.shape[0]
+        if uniform is None:
+            uniform = torch.rand(max_new_tokens, batch, generator=generator, device=input_ids.device)
+        elif tuple(uniform.shape) != (max_new_tokens, batch):
+            raise ValueError("uniform must have shape [max_new_tokens, B]")
+        empty = self.config.pad_token_id if self.config.pad_token_id is not None else 0
+        return self._generate(input_ids, max_new_tokens, graphed, lambda logits, n: sample_tokens(
+            logits, uniform[n], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, empty_token=empty))
 
 
 class GraphedDecoder:

@@ -16,7 +16,7 @@ def lib():
 
 def test_struct_sizes_match_header():
     assert ctypes.sizeof(_lib.QuantizeRowsArgs) == 16 + 5 * 8
-    assert ctypes.sizeof(_lib.Int8LinearArgs) == 8 + 6 * 4 + 11 * 8
+    assert ctypes.sizeof(_lib.Int8LinearArgs) == 8 + 6 * 4 + 11 * 8 + 8
     assert ctypes.sizeof(_lib.SampleTokensArgs) == 16 + 3 * 8 + 4 * 8 + 3 * 8 + 8 + 2 * 8
 
 
