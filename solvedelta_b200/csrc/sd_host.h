@@ -42,5 +42,15 @@ inline bool is_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() 
 // [B,T,H,w] (any outer strides, unit inner stride) or [B,T,H] -> C operand
 inline sd_operand operand(const Tensor& t) { return sd_operand{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 
+// int8 rows [N,K] as the kernels read them: 16-byte boundaries, and a row's last 16 bytes inside the storage.
+inline int64_t int8_padded(int64_t K) { return (K + 15) / 16 * 16; }
+inline bool int8_readable(const Tensor& rows) {
+    const int64_t N = rows.size(0), K = rows.size(1), stride = rows.stride(0);
+    const int64_t room = (int64_t)rows.storage().nbytes() - rows.storage_offset();
+    return (rows.stride(1) == 1 || K == 1) && (reinterpret_cast<uintptr_t>(rows.data_ptr()) & 15) == 0 &&
+           (N == 1 || (stride % 16 == 0 && stride >= int8_padded(K))) && room >= (N - 1) * stride + int8_padded(K);
+}
+inline int64_t int8_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : int8_padded(rows.size(1)); }
+
 void register_glue(py::module_& m);
 void register_serving(py::module_& m);

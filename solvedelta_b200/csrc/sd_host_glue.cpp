@@ -939,6 +939,7 @@ struct TokenLayer {
     Tensor mixer_norm, mlp_norm;
     Tensor in_weight, in_bias, conv_weight, decay_weight, gate_weight, gate_bias, log_rate, decay_bias, geometry_bias;
     Tensor out_norm, out_weight, out_bias, up_weight, down_weight;
+    Tensor up_scale, down_scale;   // the MLP's weights are int8 with these
     double mixer_eps, mlp_eps, out_eps;
     int64_t heads, width, value_width;
     Fp32Copies copies;
@@ -967,10 +968,11 @@ struct TokenStack {
                    int64_t value_width, const Tensor& in_weight, const OptTensor& in_bias, const Tensor& conv_weight,
                    const Tensor& decay_weight, const Tensor& gate_weight, const OptTensor& gate_bias, const Tensor& log_rate,
                    const Tensor& decay_bias, const Tensor& geometry_bias, const Tensor& out_norm, double out_eps,
-                   const Tensor& out_weight, const OptTensor& out_bias, const Tensor& up_weight, const Tensor& down_weight) {
+                   const Tensor& out_weight, const OptTensor& out_bias, const Tensor& up_weight, const Tensor& down_weight,
+                   const OptTensor& up_scale, const OptTensor& down_scale) {
         layers.push_back(TokenLayer{mixer_norm, mlp_norm, in_weight, given(in_bias), conv_weight, decay_weight, gate_weight,
                                     given(gate_bias), log_rate, decay_bias, geometry_bias, out_norm, out_weight, given(out_bias),
-                                    up_weight, down_weight, mixer_eps, mlp_eps, out_eps, heads, width, value_width, {}});
+                                    up_weight, down_weight, given(up_scale), given(down_scale), mixer_eps, mlp_eps, out_eps, heads, width, value_width, {}});
     }
 
     struct LayerFp32 { Tensor mixer_norm, conv, log_rate, decay_bias, geometry_bias, out_norm, mlp_norm; };
@@ -987,10 +989,18 @@ struct TokenStack {
     static bool bf16_dense(const Tensor& t, const Tensor& like) {
         return t.scalar_type() == at::kBFloat16 && t.is_contiguous() && t.device() == like.device() && aligned16(t);
     }
+    static bool int8_ok(const Tensor& w, const Tensor& scale, const Tensor& like) {
+        return w.scalar_type() == at::kChar && w.dim() == 2 && w.device() == like.device() && int8_readable(w) &&
+               scale.scalar_type() == at::kFloat && scale.device() == like.device() && scale.is_contiguous() &&
+               is_shape(scale, {w.size(0)});
+    }
     static bool weights_ok(const TokenLayer& l, const Tensor& x) {
         const int64_t D = x.size(-1), H = l.heads, r = l.width, V = l.value_width;
-        for (const Tensor* t : {&l.in_weight, &l.decay_weight, &l.gate_weight, &l.out_weight, &l.up_weight, &l.down_weight})
+        for (const Tensor* t : {&l.in_weight, &l.decay_weight, &l.gate_weight, &l.out_weight})
             if (!bf16_dense(*t, x)) return false;
+        if (l.up_scale.defined() ? !int8_ok(l.up_weight, l.up_scale, x) || !int8_ok(l.down_weight, l.down_scale, x)
+                                 : !bf16_dense(l.up_weight, x) || !bf16_dense(l.down_weight, x))
+            return false;
         for (const Tensor* t : {&l.in_bias, &l.gate_bias, &l.out_bias})
             if (t->defined() && !bf16_dense(*t, x)) return false;
         const int64_t inner = l.up_weight.size(0) / 2;
@@ -1000,7 +1010,28 @@ struct TokenStack {
                l.conv_weight.size(0) == 2 * H * r + H * V;
     }
     static bool layer_ok(const TokenLayer& l, const Tensor& x) {
-        return weights_ok(l, x) && fits_smem(x.size(0), l.up_weight.size(0) / 2) && fits_smem(x.size(0), l.heads * l.value_width);
+        return weights_ok(l, x) && (l.up_scale.defined() || fits_smem(x.size(0), l.up_weight.size(0) / 2)) && fits_smem(x.size(0), l.heads * l.value_width);
+    }
+    // x W^T on int8 weights; the scratch is shared by the launches of a call, which each wait for the one before
+    static sd_int8_linear_args int8_args(const void* in, int64_t rows, const Tensor& weight, const Tensor& scale, void* out, bool with_swiglu) {
+        sd_int8_linear_args a{};
+        a.rows = rows; a.N = (int32_t)weight.size(0); a.K = (int32_t)weight.size(1); a.swiglu = with_swiglu ? 1 : 0;
+        a.x_type = a.y_type = a.bias_type = SD_BF16;
+        a.x = in; a.x_stride = weight.size(1);
+        a.weight = weight.data_ptr(); a.weight_stride = int8_stride(weight); a.weight_scale = f32(scale);
+        a.y = out; a.y_stride = with_swiglu ? weight.size(0) / 2 : weight.size(0);
+        return a;
+    }
+    // what the rows of a call need for both products of a layer (any 16-byte aligned address stands for the activations)
+    static size_t int8_scratch(const TokenLayer& l, const Tensor& x, int64_t rows) {
+        if (!l.up_scale.defined()) return 0;
+        const sd_int8_linear_args up = int8_args(x.data_ptr(), rows, l.up_weight, l.up_scale, nullptr, true),
+                                  down = int8_args(x.data_ptr(), rows, l.down_weight, l.down_scale, nullptr, false);
+        return std::max(sd_int8_linear_scratch_bytes(&up), sd_int8_linear_scratch_bytes(&down));
+    }
+    static void int8_product(sd_int8_linear_args a, void* scratch, size_t scratch_bytes, bool chained, void* stream) {
+        a.scratch = scratch; a.scratch_bytes = scratch_bytes; a.chained = chained ? 1 : 0;
+        check(sd_int8_linear(&a, stream));
     }
     static bool fits_smem(int64_t rows, int64_t width) { return rows * (width + 96) * 2 <= 200 * 1024; }
 
@@ -1018,7 +1049,7 @@ struct TokenStack {
         // interned once and never released: a static Python object must not outlive the interpreter
         static PyObject* const recurrent_key = PyUnicode_InternFromString("recurrent_state");
         static PyObject* const conv_key = PyUnicode_InternFromString("conv_state");
-        size_t row_max = 0, y_max = 0, act_max = 0;
+        size_t row_max = 0, y_max = 0, act_max = 0, scratch_max = 0;
         for (size_t i = 0; i < layers.size(); ++i) {
             const TokenLayer& l = layers[i];
             const py::object entry = states[i];
@@ -1038,6 +1069,7 @@ struct TokenStack {
             row_max = std::max(row_max, (size_t)l.in_weight.size(0));
             y_max = std::max(y_max, (size_t)(H * V));
             act_max = std::max(act_max, (size_t)(l.up_weight.size(0) / 2));
+            scratch_max = std::max(scratch_max, int8_scratch(l, x, B));
         }
         const bool fuse_norm = B <= 16;
         if (!fuse_norm && (D % 256 != 0)) return std::nullopt;   // the norm alone takes whole groups of 256 channels
@@ -1049,10 +1081,11 @@ struct TokenStack {
         const Tensor last_norm = copies.get(0, norm);
         const auto piece = [&](size_t width) { return (width * (size_t)B * 2 + 255) & ~size_t(255); };
         const size_t row_b = piece(row_max), y_b = piece(y_max), act_b = piece(act_max), d_b = piece((size_t)D);
-        const Tensor work = workspace(x, row_b + y_b + act_b + 5 * d_b);
+        const Tensor work = workspace(x, row_b + y_b + act_b + 5 * d_b + scratch_max);
         char* base = static_cast<char*>(work.data_ptr());
         char *row = base, *y = row + row_b, *act = y + y_b, *mixed = act + act_b, *mlp = mixed + d_b, *normed = mlp + d_b;
         char* sums[2] = {normed + d_b, normed + 2 * d_b};
+        char* const scratch = sums[1] + d_b;
         int next = 0;
         const void* residual = x.data_ptr();
         const void* delta = nullptr;
@@ -1136,8 +1169,15 @@ struct TokenStack {
             check(sd_mixer_decode_step_chained(&a, stream));
             linear(y, H * V, l.out_weight, raw(l.out_bias), mixed, false, nullptr, 0);
             delta = mixed;
-            norm_linear(f32(w.mlp_norm), l.mlp_eps, l.up_weight, nullptr, act, true);
-            linear(act, l.up_weight.size(0) / 2, l.down_weight, nullptr, mlp, false, nullptr, 0);
+            if (l.up_scale.defined()) {
+                norm_rows(f32(w.mlp_norm), l.mlp_eps, normed);
+                int8_product(int8_args(normed, B, l.up_weight, l.up_scale, act, true), scratch, scratch_max, true, stream);
+                int8_product(int8_args(act, B, l.down_weight, l.down_scale, mlp, false), scratch, scratch_max, true, stream);
+                chained = true;
+            } else {
+                norm_linear(f32(w.mlp_norm), l.mlp_eps, l.up_weight, nullptr, act, true);
+                linear(act, l.up_weight.size(0) / 2, l.down_weight, nullptr, mlp, false, nullptr, 0);
+            }
             delta = mlp;
         }
         Tensor out = bf16_like(x, {B, 1, head.has_value() ? head->size(0) : D});
@@ -1170,7 +1210,8 @@ struct TokenStack {
             const Plan pl{up256(sd_inference_bytes(&sh)), up256(sd_forward_scratch_bytes(&sh))};
             const size_t mixer = bf16_rows(l.in_weight.size(0)) + bf16_rows(2 * H * r + H * V) + 3 * bf16_rows(H * r) + bf16_rows(2 * H) +
                                  3 * bf16_rows(H * V) + pl.saved + pl.scratch;
-            area = std::max({area, mixer, bf16_rows(l.up_weight.size(0)) + bf16_rows(l.up_weight.size(0) / 2)});
+            const size_t inner = bf16_rows(l.up_weight.size(0) / 2);
+            area = std::max({area, mixer, l.up_scale.defined() ? inner + int8_scratch(l, x, R) : bf16_rows(l.up_weight.size(0)) + inner});
             plan.push_back(pl);
         }
         const c10::cuda::CUDAGuard guard(x.device());
@@ -1252,12 +1293,19 @@ struct TokenStack {
             delta = mixed;
             norm_rows(w32.mlp_norm, l.mlp_eps, normed);
             const int64_t inner = l.up_weight.size(0) / 2;
-            char *up = base, *act = base + bf16_rows(2 * inner);
-            linear(normed, D, l.up_weight, Tensor(), up);
-            sd_swiglu_args w{};
-            w.I = (int32_t)inner; w.rows = R; w.gate_value = up; w.out = act;
-            check(sd_swiglu(&w, stream));
-            linear(act, inner, l.down_weight, Tensor(), mlp);
+            if (l.up_scale.defined()) {
+                char* const scratch = base + bf16_rows(inner);
+                const size_t bytes = int8_scratch(l, x, R);
+                int8_product(int8_args(normed, R, l.up_weight, l.up_scale, base, true), scratch, bytes, false, stream);
+                int8_product(int8_args(base, R, l.down_weight, l.down_scale, mlp, false), scratch, bytes, true, stream);
+            } else {
+                char *up = base, *act = base + bf16_rows(2 * inner);
+                linear(normed, D, l.up_weight, Tensor(), up);
+                sd_swiglu_args w{};
+                w.I = (int32_t)inner; w.rows = R; w.gate_value = up; w.out = act;
+                check(sd_swiglu(&w, stream));
+                linear(act, inner, l.down_weight, Tensor(), mlp);
+            }
             delta = mlp;
             if (want_states) states.append(py::make_tuple(C, S, window));
         }

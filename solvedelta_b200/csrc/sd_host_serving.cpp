@@ -5,7 +5,6 @@
 
 namespace {
 
-int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
 int element_type(const Tensor& t) { return t.scalar_type() == at::kFloat ? SD_F32 : SD_BF16; }
 bool is_real(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 
@@ -17,19 +16,13 @@ Tensor as_rows(const Tensor& t) {
 }
 int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : std::max<int64_t>(rows.stride(0), rows.size(1)); }
 
-// int8 rows as the kernels read them: 16-byte boundaries, and a row's last 16 bytes inside the storage.  Rows that
-// quantize_rows made are; others are copied.
+// Rows that quantize_rows made are read in place; others are copied.
 Tensor readable(const Tensor& rows) {
-    const int64_t N = rows.size(0), K = rows.size(1), need = padded(K), stride = rows.stride(0);
-    const int64_t room = (int64_t)rows.storage().nbytes() - rows.storage_offset();
-    if ((rows.stride(1) == 1 || K == 1) && (reinterpret_cast<uintptr_t>(rows.data_ptr()) & 15) == 0 &&
-        (N == 1 || (stride % 16 == 0 && stride >= need)) && room >= (N - 1) * stride + need)
-        return rows;
-    Tensor copy = at::empty({N, need}, rows.options());
-    copy.narrow(1, 0, K).copy_(rows);
-    return copy.narrow(1, 0, K);
+    if (int8_readable(rows)) return rows;
+    Tensor copy = at::empty({rows.size(0), int8_padded(rows.size(1))}, rows.options()).narrow(1, 0, rows.size(1));
+    copy.copy_(rows);
+    return copy;
 }
-int64_t int8_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : padded(rows.size(1)); }
 
 void require_no_gradient(std::initializer_list<const Tensor*> tensors) {
     if (!at::GradMode::is_enabled()) return;
@@ -52,15 +45,15 @@ py::tuple quantize_rows(const Tensor& x) {
     const Tensor rows = as_rows(x.detach());
     const int64_t M = rows.size(0);
     value_error(M > 0x7fffffffLL, "too many rows");
-    Tensor q = at::empty({M, padded(K)}, x.options().dtype(at::kChar)), scale = f32_like(x, {M});
+    Tensor q = at::empty({M, int8_padded(K)}, x.options().dtype(at::kChar)), scale = f32_like(x, {M});
     if (M > 0) {
         sd_quantize_rows_args a{};
         a.rows = M; a.K = (int32_t)K; a.x_type = element_type(rows); a.x = rows.data_ptr(); a.x_stride = row_stride(rows);
-        a.q = q.data_ptr(); a.q_stride = padded(K); a.scale = f32(scale);
+        a.q = q.data_ptr(); a.q_stride = int8_padded(K); a.scale = f32(scale);
         check(sd_quantize_rows(&a, stream_of(x)));
     }
     std::vector<int64_t> shape = x.sizes().vec(), stride(shape.size(), 1);
-    int64_t step = padded(K);
+    int64_t step = int8_padded(K);
     for (int64_t d = (int64_t)shape.size() - 2; d >= 0; --d) {
         stride[d] = step;
         step *= std::max<int64_t>(shape[d], 1);

@@ -17,6 +17,7 @@ from torch import nn
 from torch.nn.modules import module as module_globals
 
 from . import _lib, model as mixer_module
+from .int8_ops import Int8Linear
 from .model import RMSNormGated, SolveDelta
 
 _STACKS: "weakref.WeakKeyDictionary" = weakref.WeakKeyDictionary()
@@ -43,7 +44,9 @@ def _build(model, block_type, adapter_type, mlp_type):
         watched += [(block, block_type), (block.mixer, adapter_type), (mixer, SolveDelta), (mlp, mlp_type),
                     (block.mixer_norm, nn.RMSNorm), (block.mlp_norm, nn.RMSNorm), (mixer.output_norm, RMSNormGated)]
         watched += [(linear, nn.Linear) for linear in (mixer.in_proj, mixer.decay_proj, mixer.output_gate_proj,
-                                                       mixer.output_proj, mlp.gate_up_proj, mlp.down_proj)]
+                                                       mixer.output_proj)]
+        kind = Int8Linear if type(mlp.gate_up_proj) is Int8Linear else nn.Linear   # both in int8, or none
+        watched += [(mlp.gate_up_proj, kind), (mlp.down_proj, kind)]
         if (any(type(m) is not t for m, t in watched) or mlp.gate_up_proj.bias is not None
                 or mlp.down_proj.bias is not None or block.mixer_norm.weight is None or block.mlp_norm.weight is None):
             return None
@@ -54,9 +57,10 @@ def _build(model, block_type, adapter_type, mlp_type):
             mixer.in_proj.weight, mixer.in_proj.bias, mixer.conv_weight, mixer.decay_proj.weight,
             mixer.output_gate_proj.weight, mixer.output_gate_proj.bias, mixer.associative_log_rate,
             mixer.associative_decay_bias, mixer.geometry_write_bias, mixer.output_norm.weight, mixer.output_norm.eps,
-            mixer.output_proj.weight, mixer.output_proj.bias, mlp.gate_up_proj.weight, mlp.down_proj.weight)
+            mixer.output_proj.weight, mixer.output_proj.bias, mlp.gate_up_proj.weight, mlp.down_proj.weight,
+            getattr(mlp.gate_up_proj, "weight_scale", None), getattr(mlp.down_proj, "weight_scale", None))
     for module, _ in watched:
-        for children in (module._modules, module._parameters):
+        for children in (module._modules, module._parameters, module._buffers):
             for name, child in children.items():
                 stack.watch_same(children, name, child)
         if "eps" in module.__dict__:
