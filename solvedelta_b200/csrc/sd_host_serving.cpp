@@ -8,6 +8,9 @@ namespace {
 int element_type(const Tensor& t) { return t.scalar_type() == at::kFloat ? SD_F32 : SD_BF16; }
 bool is_real(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 
+// The calls record nothing, and skip autograd's part of every tensor operation (about a tenth of a short call each).
+using NoAutograd = at::AutoDispatchBelowADInplaceOrView;
+
 // [..., K] as rows with unit channel stride and one stride between them; a view where the layout has that.
 Tensor as_rows(const Tensor& t) {
     const int64_t K = t.size(-1);
@@ -42,25 +45,31 @@ py::tuple quantize_rows(const Tensor& x) {
     const int64_t K = x.size(-1);
     check_width(K);
     const c10::cuda::CUDAGuard guard(x.device());
-    const Tensor rows = as_rows(x.detach());
+    const NoAutograd below;
+    const Tensor rows = as_rows(x);
     const int64_t M = rows.size(0);
     value_error(M > 0x7fffffffLL, "too many rows");
-    Tensor q = at::empty({M, int8_padded(K)}, x.options().dtype(at::kChar)), scale = f32_like(x, {M});
+    const int64_t pitch = int8_padded(K);
+    std::vector<int64_t> shape = x.sizes().vec();
+    const bool dense = pitch == K;   // else the rows' padding is cut off below
+    Tensor q = dense ? at::empty(shape, x.options().dtype(at::kChar)) : at::empty({M, pitch}, x.options().dtype(at::kChar));
+    Tensor scale = f32_like(x, x.sizes().slice(0, x.dim() - 1));
     if (M > 0) {
         sd_quantize_rows_args a{};
         a.rows = M; a.K = (int32_t)K; a.x_type = element_type(rows); a.x = rows.data_ptr(); a.x_stride = row_stride(rows);
-        a.q = q.data_ptr(); a.q_stride = int8_padded(K); a.scale = f32(scale);
+        a.q = q.data_ptr(); a.q_stride = pitch; a.scale = f32(scale);
         check(sd_quantize_rows(&a, stream_of(x)));
     }
-    std::vector<int64_t> shape = x.sizes().vec(), stride(shape.size(), 1);
-    int64_t step = int8_padded(K);
-    for (int64_t d = (int64_t)shape.size() - 2; d >= 0; --d) {
-        stride[d] = step;
-        step *= std::max<int64_t>(shape[d], 1);
+    if (!dense) {
+        std::vector<int64_t> stride(shape.size(), 1);
+        int64_t step = pitch;
+        for (int64_t d = (int64_t)shape.size() - 2; d >= 0; --d) {
+            stride[d] = step;
+            step *= std::max<int64_t>(shape[d], 1);
+        }
+        q = q.as_strided(shape, stride);
     }
-    q = q.as_strided(shape, stride);
-    shape.pop_back();
-    return py::make_tuple(q, scale.view(shape));
+    return py::make_tuple(q, scale);
 }
 
 at::ScalarType output_type(const py::object& dtype) {
@@ -94,21 +103,22 @@ Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in,
     require_no_gradient({&x, &scale_in, &weight_scale_in, &bias});
 
     const c10::cuda::CUDAGuard guard(x.device());
+    const NoAutograd below;
     std::vector<int64_t> shape = x.sizes().vec();
     if (quantized) {
         type_error(scale_in.scalar_type() != at::kFloat, "scale must be FP32");
         value_error(!is_shape(scale_in, x.sizes().slice(0, x.dim() - 1)), "scale must have the shape of the rows without their last axis");
     }
-    Tensor rows = as_rows(x.detach());
+    Tensor rows = as_rows(x);
     const int64_t M = rows.size(0);
     value_error(M > 0x7fffff00LL, "too many rows");
     shape.back() = swiglu ? N / 2 : N;
     Tensor y = at::empty(shape, x.options().dtype(out_type));
     if (M == 0) return y;
     if (quantized) rows = readable(rows);
-    const Tensor weight = readable(weight_in.detach()), weight_scale = weight_scale_in.detach().contiguous();
-    const Tensor scale = quantized ? scale_in.detach().reshape({M}).contiguous() : Tensor();
-    const Tensor b = bias.defined() ? bias.detach().contiguous() : Tensor();
+    const Tensor weight = readable(weight_in), weight_scale = weight_scale_in.contiguous();
+    const Tensor scale = !quantized ? Tensor() : scale_in.is_contiguous() ? scale_in : scale_in.contiguous();
+    const Tensor b = bias.defined() ? bias.contiguous() : Tensor();
     // a copy made here is written by the kernel before
     chained = chained && weight.data_ptr() == weight_in.data_ptr() && weight_scale.data_ptr() == weight_scale_in.data_ptr() &&
               (!b.defined() || b.data_ptr() == bias.data_ptr());
@@ -154,8 +164,8 @@ Tensor row_setting(const py::object& value, const char* name, const Tensor& logi
     if (t.device() != logits.device()) throw py::value_error(std::string(name) + " must be on the device of the logits");
     if (type == at::kInt ? !at::isIntegralType(t.scalar_type(), false) : !at::isFloatingType(t.scalar_type()))
         throw py::type_error(std::string(name) + (type == at::kInt ? " must hold whole numbers" : " must hold real numbers"));
-    if (type == at::kInt && t.scalar_type() == at::kLong) return t.detach().clamp(0, 0x7fffffff).to(type).contiguous();
-    return t.detach().to(type).contiguous();
+    if (type == at::kInt && t.scalar_type() == at::kLong) return t.clamp(0, 0x7fffffff).to(type).contiguous();
+    return t.to(type).contiguous();
 }
 
 Tensor sample_tokens(const Tensor& logits_in, const Tensor& uniform, const py::object& temperature, const py::object& top_k,
@@ -167,7 +177,8 @@ Tensor sample_tokens(const Tensor& logits_in, const Tensor& uniform, const py::o
     type_error(uniform.scalar_type() != at::kFloat, "uniform must be FP32");
     value_error(!is_shape(uniform, {B}) || uniform.device() != logits_in.device(), "uniform must be [B] on the device of the logits");
     const c10::cuda::CUDAGuard guard(logits_in.device());
-    const Tensor logits = as_rows(logits_in.detach()), u = uniform.detach().contiguous();
+    const NoAutograd below;
+    const Tensor logits = as_rows(logits_in), u = uniform.contiguous();
     const Tensor t = row_setting(temperature, "temperature", logits, at::kFloat), k = row_setting(top_k, "top_k", logits, at::kInt),
                  tp = row_setting(top_p, "top_p", logits, at::kFloat), mp = row_setting(min_p, "min_p", logits, at::kFloat);
     sd_sample_tokens_args a{};
