@@ -303,6 +303,40 @@ __device__ __forceinline__ void int8_store(const Int8Params& p, unsigned char* s
     }
 }
 
+// The scales and biases of a tile's weight rows, by the epilogue's threads (OUTS output columns from column0 on; with GATED the
+// value rows' behind them).
+template <int BN, bool GATED>
+__device__ __forceinline__ void int8_columns(const Int8Params& p, int column0, float* scale, float* bias) {
+    constexpr int OUTS = GATED ? BN / 2 : BN;
+    const int i = threadIdx.x - I8_EPILOGUE_WARP * 32;
+    if (i >= BN) return;
+    const int col = column0 + (GATED ? i % OUTS : i), w = GATED && i >= OUTS ? p.outs + col : col;
+    scale[i] = col < p.outs ? p.w_scale[w] : 0.f;
+    bias[i] = col < p.outs ? int8_bias(p, w) : 0.f;
+}
+// A row's sums v (and g, of the value rows) of STEP columns from c0 of the tile on -> outputs in v.
+template <int STEP, bool GATED>
+__device__ __forceinline__ void int8_finish(const Int8Params& p, float (&v)[STEP], float (&g)[GATED ? STEP : 1], float sx, const float* scale,
+                                            const float* bias, int c0, int values) {
+    // (shared memory is what the products are short of: without a bias none is read)
+#pragma unroll
+    for (int e = 0; e < STEP; ++e) {
+        v[e] = (float)__float_as_int(v[e]) * sx * scale[c0 + e];
+        if constexpr (GATED) g[e] = (float)__float_as_int(g[e]) * sx * scale[values + c0 + e];
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+        for (int e = 0; e < STEP; ++e) {
+            v[e] += bias[c0 + e];
+            if constexpr (GATED) g[e] += bias[values + c0 + e];
+        }
+    }
+    if constexpr (GATED) {
+#pragma unroll
+        for (int e = 0; e < STEP; ++e) v[e] = int8_gated(v[e], g[e]);
+    }
+}
+
 template <int BN, bool GATED, bool F32, bool PAIR>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, int* fault) {
@@ -422,7 +456,7 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
         }
         __syncwarp();
     } else if (warp >= I8_EPILOGUE_WARP) {   // ---- scales, bias, gate, store
-        const int quarter = warp & 3, half = (warp - I8_EPILOGUE_WARP) >> 2, etid = tid - I8_EPILOGUE_WARP * 32;
+        const int quarter = warp & 3, half = (warp - I8_EPILOGUE_WARP) >> 2;
         const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.y_stride % (F32 ? 4 : 8) == 0;
         int t = 0;
         bool alive = true;
@@ -430,12 +464,7 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
             int m, n;
             place(tile, m, n);
             float *scale = s_scale[t & 1], *bias = s_bias[t & 1];
-            if (etid < BN) {
-                const int c = GATED ? etid % OUTS : etid, col = n * OUTS + c;
-                const int w = GATED && etid >= OUTS ? p.outs + col : col;
-                scale[etid] = col < p.outs ? p.w_scale[w] : 0.f;
-                bias[etid] = col < p.outs ? int8_bias(p, w) : 0.f;
-            }
+            int8_columns<BN, GATED>(p, n * OUTS, scale, bias);
             asm volatile("bar.sync 1, %0;" ::"n"(I8_EPILOGUE_THREADS) : "memory");
             const int row0 = m * BM + rank * I8_BM + quarter * 32;
             const float sx = row0 + lane < p.M ? p.x_scale[row0 + lane] : 0.f;
@@ -455,23 +484,7 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
                 tc_ld<STEP>(acc + c0, v);
                 if constexpr (GATED) tc_ld<STEP>(acc + OUTS + c0, g);
                 tc_wait_ld();
-                // (shared memory is what the products are short of: without a bias none is read)
-#pragma unroll
-                for (int e = 0; e < STEP; ++e) {
-                    v[e] = (float)__float_as_int(v[e]) * sx * scale[c0 + e];
-                    if constexpr (GATED) g[e] = (float)__float_as_int(g[e]) * sx * scale[OUTS + c0 + e];
-                }
-                if (p.bias != nullptr) {
-#pragma unroll
-                    for (int e = 0; e < STEP; ++e) {
-                        v[e] += bias[c0 + e];
-                        if constexpr (GATED) g[e] += bias[OUTS + c0 + e];
-                    }
-                }
-                if constexpr (GATED) {
-#pragma unroll
-                    for (int e = 0; e < STEP; ++e) v[e] = int8_gated(v[e], g[e]);
-                }
+                int8_finish<STEP, GATED>(p, v, g, sx, scale, bias, c0, OUTS);
                 int8_store<F32>(p, staging, row0, n * OUTS + c0, v, vec);
             }
             tc_fence_before();
@@ -487,6 +500,148 @@ k_int8_matmul(Int8Params p, const __grid_constant__ CUtensorMap x_map, const __g
         else
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(Tile::TMEM_COLS));
     }
+}
+
+// The same product where tiles of 128 x 64 are too few for the SMs and the sums are long: the 2, 4 or 8 CTAs of a cluster take
+// a tile together, a part of K each (one SM receives some 40 bytes a clock, so that K = 5632 takes it 14 us alone).  Then each
+// gets every CTA's sums of its own 64 / CTAS columns, in its ring, which is free by then, adds them up, exactly, and stores.
+constexpr int I8_SPLIT_BN = 64;
+
+template <bool GATED, bool F32>
+__global__ void __launch_bounds__(I8_THREADS, 1)
+k_int8_split(Int8Params p, int ctas_log2, int per, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, int* fault) {
+    using Tile = Int8Tile<I8_SPLIT_BN, false>;
+    constexpr int S = Tile::STAGES, BN = I8_SPLIT_BN, OUTS = GATED ? BN / 2 : BN;
+    extern __shared__ __align__(16) unsigned char i8_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * S + 1];   // full, empty, accumulator full
+    __shared__ unsigned s_tmem;
+    __shared__ __align__(16) float s_scale[BN], s_bias[BN];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = 1 << ctas_log2, rank = blockIdx.x & (ctas - 1),
+              tile = blockIdx.x >> ctas_log2;
+    const unsigned ring = (tc_smem(i8_raw) + 1023u) & ~1023u;
+    unsigned char* const parts = i8_raw + (ring - tc_smem(i8_raw));
+    const unsigned full0 = tc_smem(bars), empty0 = full0 + 8 * S, acc_full = empty0 + 8 * S;
+    const auto everywhere = [] { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); };
+
+    if (tid == 0) {
+        for (int i = 0; i < 2 * S + 1; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8 * i));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&s_tmem)), "r"(BN));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    if (warp == 3 && lane < 2)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(lane == 0 ? &x_map : &w_map)) : "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    chain_wait();
+    chain_release();
+    const unsigned tbase = s_tmem;
+    const int m = tile % p.tiles_m, n = tile / p.tiles_m;
+    const int blocks = (p.K + I8_BK - 1) / I8_BK, first = rank * per, count = min(per, blocks - first);   // none: nothing is added
+    const int quarter = warp & 3, half = (warp - I8_EPILOGUE_WARP) >> 2, row0 = m * I8_BM + quarter * 32;
+    const bool epilogue = warp >= I8_EPILOGUE_WARP;
+    bool alive = true;
+
+    if (warp == 0 && lane == 0) {
+        int k = 0;
+        for (; k < count; ++k) {
+            const int s = k % S;
+            if (k >= S) alive = tc_wait(empty0 + 8 * s, (k / S - 1) & 1);
+            if (!alive) break;
+            const unsigned bar = full0 + 8 * s, a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(Tile::STAGE_BYTES) : "memory");
+            i8_load<false>(a, &x_map, (first + k) * I8_BK, m * I8_BM, bar);
+            i8_load<false>(w, &w_map, (first + k) * I8_BK, n * OUTS, bar);
+            if (GATED) i8_load<false>(w + Tile::B_BYTES / 2, &w_map, (first + k) * I8_BK, p.outs + n * OUTS, bar);
+        }
+        if (!alive) {
+            atomicExch(fault, 9);
+            for (int i = k > S ? k - S : 0; i < k; ++i) tc_wait(full0 + 8 * (i % S), (i / S) & 1);   // copies in flight
+        }
+    } else if (warp == 1 && lane == 0) {
+        for (int k = 0; k < count && alive; ++k) {
+            const int s = k % S;
+            alive = tc_wait(full0 + 8 * s, (k / S) & 1);
+            if (!alive) break;
+            tc_fence_after();
+            const unsigned a = ring + s * Tile::STAGE_BYTES, w = a + Tile::A_BYTES;
+#pragma unroll
+            for (int j = 0; j < I8_BK / 32; ++j)
+                i8_mma<false>(tbase, tc_desc(a + j * 32, 16, 1024) | (2ull << 61), tc_desc(w + j * 32, 16, 1024) | (2ull << 61),
+                              i8_idesc(I8_BM, BN), k > 0 || j > 0 ? 1u : 0u);
+            i8_commit<false>(empty0 + 8 * s);
+        }
+        if (alive && count > 0) i8_commit<false>(acc_full);
+        if (!alive) atomicExch(fault, 10);
+    } else if (epilogue) {
+        int8_columns<BN, GATED>(p, n * OUTS, s_scale, s_bias);
+        alive = count <= 0 || tc_wait(acc_full, 0);
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive && lane == 0) atomicExch(fault, 11);
+        tc_fence_after();
+    }
+    __syncwarp();
+    everywhere();   // all products are done: the rings are free
+    // A CTA's part: from every CTA `width` columns of 128 rows; with GATED half of them gate and half value columns.
+    const int width_log2 = 6 - ctas_log2, width = 1 << width_log2, half_log2 = width_log2 - (GATED ? 1 : 0);
+    if (epilogue && alive && count > 0 && row0 < p.M) {
+        float v[32];
+        tc_ld32(tbase + ((unsigned)(quarter * 32) << 16) + half * 32, v);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const int col = half * 32 + e, in = GATED ? e : col;   // column of the tile, and among the gates (values)
+            const int to = in >> half_log2, local = (in & ((1 << half_log2) - 1)) + (GATED && half == 1 ? width / 2 : 0);
+            unsigned at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                         : "=r"(at)
+                         : "r"(ring + (((rank << width_log2) + local) * I8_BM + quarter * 32 + lane) * 4), "r"(to));
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "f"(v[e]) : "memory");
+        }
+    }
+    everywhere();
+    const int outs = GATED ? width / 2 : width, col0 = rank * outs;   // of the tile
+    if (epilogue && alive && row0 + lane < p.M) {
+        const int row = row0 + lane;
+        const float sx = p.x_scale[row];
+        const int* part = reinterpret_cast<const int*>(parts) + quarter * 32 + lane;
+        const int active = (blocks + per - 1) / per;
+        const auto sum = [&](int local) {
+            int v = 0;
+            for (int r = 0; r < active; ++r) v += part[((r << width_log2) + local) * I8_BM];
+            return (float)v * sx;
+        };
+        constexpr int STEP = 2;   // neighbouring columns, one store where rows allow it
+        const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 && p.y_stride % STEP == 0;
+        for (int c = half * STEP; c < outs; c += 2 * STEP) {
+            float v[STEP];
+#pragma unroll
+            for (int e = 0; e < STEP; ++e) {
+                const int i = col0 + c + e;
+                v[e] = sum(c + e) * s_scale[i] + s_bias[i];
+                if constexpr (GATED) v[e] = int8_gated(v[e], sum(outs + c + e) * s_scale[OUTS + i] + s_bias[OUTS + i]);
+            }
+            const int col = n * OUTS + col0 + c;
+            const long long at = row * p.y_stride + col;
+            if constexpr (F32) {
+                float* y = reinterpret_cast<float*>(p.y) + at;
+                if (vec && col + STEP <= p.outs) *reinterpret_cast<float2*>(y) = make_float2(v[0], v[1]);
+                else
+                    for (int e = 0; e < STEP && col + e < p.outs; ++e) y[e] = v[e];
+            } else {
+                __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + at;
+                if (vec && col + STEP <= p.outs) *reinterpret_cast<__nv_bfloat162*>(y) = __floats2bfloat162_rn(v[0], v[1]);
+                else
+                    for (int e = 0; e < STEP && col + e < p.outs; ++e) y[e] = __float2bfloat16_rn(v[e]);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(BN));
 }
 
 // ---- few rows: a cached token of a serving batch --------------------------------------------------------------------

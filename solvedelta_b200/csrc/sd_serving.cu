@@ -114,6 +114,27 @@ int launch_matmul(Int8Params p, const sd_int8_linear_args* a, const void* q, lon
     return launch<k_int8_matmul<BN, GATED, F32, PAIR>>(workers * CTAS, I8_THREADS, Int8Tile<BN, PAIR>::SMEM, Int8Tile<BN, PAIR>::SMEM, CTAS,
                                                        chained, stream, p, x_map, w_map, fault);
 }
+// How many CTAs share a tile of 128 x 64 (as a power of two): as many as the SMs have room for, four steps of K each at least.
+int split_log2(long long tiles, int K) {
+    const int blocks = (K + I8_BK - 1) / I8_BK;
+    int n = 0;
+    while (n < 3 && (tiles << (n + 1)) <= 148 && blocks >> (n + 1) >= 4) ++n;
+    return n;
+}
+template <bool GATED, bool F32>
+int launch_split(Int8Params p, const sd_int8_linear_args* a, const void* q, long long q_stride, int ctas_log2, bool chained, cudaStream_t stream) {
+    using Tile = Int8Tile<I8_SPLIT_BN, false>;
+    constexpr int OUTS = GATED ? I8_SPLIT_BN / 2 : I8_SPLIT_BN;
+    CUtensorMap x_map, w_map;
+    int* fault = fault_word();
+    if (fault == nullptr) return SD_ERR_NO_DEVICE;
+    if (!int8_map(&x_map, q, p.M, p.K, q_stride, I8_BM) || !int8_map(&w_map, a->weight, a->N, p.K, a->weight_stride, OUTS)) return SD_ERR_LAUNCH_FAILED;
+    p.tiles_m = (p.M + I8_BM - 1) / I8_BM;
+    p.tiles_n = (p.outs + OUTS - 1) / OUTS;
+    const int blocks = (p.K + I8_BK - 1) / I8_BK, ctas = 1 << ctas_log2, per = (blocks + ctas - 1) / ctas;
+    return launch<k_int8_split<GATED, F32>>((unsigned)(p.tiles_m * p.tiles_n * ctas), I8_THREADS, Tile::SMEM, Tile::SMEM, ctas, chained, stream, p,
+                                            ctas_log2, per, x_map, w_map, fault);
+}
 template <bool GATED, bool F32>
 int matmul_tile(const Int8Params& p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
     const auto tiles = [&](int bm, int bn) {
@@ -123,6 +144,8 @@ int matmul_tile(const Int8Params& p, const sd_int8_linear_args* a, const void* q
     // the widest tile that still gives every SM one
     if (tiles(256, 256) >= 74 && p.M > 128) return launch_matmul<256, GATED, F32, true>(p, a, q, q_stride, chained, stream);
     if (tiles(128, 128) >= 148) return launch_matmul<128, GATED, F32, false>(p, a, q, q_stride, chained, stream);
+    const int ctas_log2 = split_log2(tiles(128, 64), p.K);
+    if (ctas_log2 > 0) return launch_split<GATED, F32>(p, a, q, q_stride, ctas_log2, chained, stream);
     return launch_matmul<64, GATED, F32, false>(p, a, q, q_stride, chained, stream);
 }
 int matmul(const Int8Params& p, const sd_int8_linear_args* a, const void* q, long long q_stride, bool chained, cudaStream_t stream) {
