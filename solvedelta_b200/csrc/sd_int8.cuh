@@ -647,13 +647,13 @@ k_int8_split(Int8Params p, int ctas_log2, int per, const __grid_constant__ CUten
 // ---- few rows: a cached token of a serving batch --------------------------------------------------------------------
 // Bound by the weight, read once, and behind that by the latency of one launch.  Two CTAs of eight warps per SM stay for
 // all their tiles of 8 CG weight rows (gate and value rows side by side with SwiGLU).  A warp takes one group of eight
-// weight rows and a slice of K; a lane keeps the 16-byte pieces of two steps in flight ahead of the products.  The products
+// weight rows and a slice of K; a lane keeps the 16-byte pieces of three steps in flight ahead of the products.  The products
 // run on mma.sync m16n8k32 with the rows of x as the M side: the contraction index is permuted so that a lane's 16-byte
 // piece of a weight row is its B fragment of two instructions, and the rows, in shared memory, are read with the same
 // permutation.  BF16 rows are quantised by every CTA on the way into shared memory.
-constexpr int I8_TOKEN_ROWS = 32;
+constexpr int I8_TOKEN_ROWS = 16;   // past that the tensor-memory kernels take less (24 x 1024 x 7488: 7.6 us against 9.8)
 constexpr size_t I8_TOKEN_SMEM = 190 * 1024;
-constexpr int I8_TOKEN_BATCH = 4;
+constexpr int I8_TOKEN_BATCH = 4, I8_TOKEN_AHEAD = 3;   // weight pieces per lane and step, steps in flight
 // Row pitch in shared memory, 64 bytes off a multiple of 128: the eight 16-byte pieces a quarter-warp reads (two rows, four
 // consecutive pieces) fall into distinct banks.
 __host__ __device__ constexpr long long int8_pitch(int K) { return ((long long)K + 127) / 128 * 128 + 64; }
@@ -731,7 +731,7 @@ __device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char*
 
 // RG: groups of eight rows; CG: groups of eight weight rows per CTA (2 with GATED)
 template <int RG, int CG, bool GATED, class T, bool VEC>
-__global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenParams p) {
+__global__ void __launch_bounds__(256, 2) k_int8_token(Int8TokenParams p) {
     static_assert(!GATED || CG == 2, "gate and value rows are the two groups");
     constexpr int KS = 8 / CG, MT = (RG + 1) / 2, B = I8_TOKEN_BATCH;
     extern __shared__ __align__(16) unsigned char i8_raw[];
@@ -746,24 +746,32 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
     const int chunks = (K + 63) / 64, per = (chunks + KS - 1) / KS;
     const int begin = min(ks * per, chunks), end = min(begin + per, chunks);
     const int steps = (per + B - 1) / B;
-    const int mine = tiles > (int)blockIdx.x ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-    const int total = mine * steps;
     const int pitch = (int)int8_pitch(K);
 
-    const auto request = [&](int item, uint4 (&w)[B]) {
-        const int tile = blockIdx.x + item / steps * gridDim.x, base = begin + item % steps * B;
-        const int col = tile * WIDTH + (GATED ? g : cg * 8 + g);
-        const bool ok = item < total && col < outs;
-        const signed char* row = p.W + (long long)(GATED ? col + cg * outs : col) * p.w_stride + t * 16;
+    // The next step to be requested: its tile, its number there, and its first pieces.  (Counted on; a division per step was a
+    // third of the instructions.)
+    int want_tile = blockIdx.x, want_step = 0;
+    const signed char* want = nullptr;
+    bool want_live = false;
+    const auto request = [&](uint4 (&w)[B]) {
+        if (want_step == 0) {
+            const int col = want_tile * WIDTH + (GATED ? g : cg * 8 + g);
+            want_live = want_tile < tiles && col < outs;
+            want = p.W + (long long)(GATED ? col + cg * outs : col) * p.w_stride + begin * 64 + t * 16;
+        }
+        const int base = begin + want_step * B;
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const int c = base + i;
-            w[i] = ok && c < end && c * 64 + t * 16 < K ? load_weight(row + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < B; ++i)
+            w[i] = want_live && base + i < end && (base + i) * 64 + t * 16 < K ? load_weight(want + i * 64) : make_uint4(0u, 0u, 0u, 0u);
+        want += B * 64;
+        if (++want_step == steps) {
+            want_step = 0;
+            want_tile += gridDim.x;
         }
     };
-    uint4 wa[B], wb[B];
-    request(0, wa);
-    request(1, wb);
+    uint4 w[I8_TOKEN_AHEAD][B];
+#pragma unroll
+    for (int i = 0; i < I8_TOKEN_AHEAD; ++i) request(w[i]);
     chain_wait();
     chain_release();
     int8_rows<T, VEC>(p, s_q, s_scale, s_top);
@@ -781,10 +789,11 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
         }
     };
     int acc[MT][4];
-    const auto step = [&](int item, uint4 (&w)[B]) {
-        const int st = item % steps, base = begin + st * B;
+    int tile = blockIdx.x, st = 0, buf = 0;
+    const auto step = [&](uint4 (&w)[B]) {
+        const int base = begin + st * B;
         if (st == 0) {
-            finish_of(blockIdx.x + item / steps * gridDim.x);   // requested ahead of the products
+            finish_of(tile);   // requested ahead of the products
 #pragma unroll
             for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -804,10 +813,9 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
                 }
             }
         }
-        request(item + 2, w);
-        if (st != steps - 1) return;
+        request(w);
+        if (++st != steps) return;
         // last step of a tile: the K slices are added up through shared memory (two buffers in turn, so one barrier)
-        const int tile_no = item / steps, buf = tile_no & 1;
 #pragma unroll
         for (int a = 0; a < MT; ++a) {
             s_red[buf][warp][a * 16 + g][2 * t] = acc[a][0];
@@ -818,7 +826,7 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
             }
         }
         __syncthreads();
-        const int n = (blockIdx.x + tile_no * gridDim.x) * WIDTH + out_col;
+        const int n = tile * WIDTH + out_col;
         for (int m = tid / WIDTH; m < M && n < outs; m += 256 / WIDTH) {
             const auto value = [&](int group, int j) {
                 int v = 0;
@@ -831,10 +839,14 @@ __global__ void __launch_bounds__(256, RG <= 2 ? 2 : 1) k_int8_token(Int8TokenPa
             if (p.o.out_f32) reinterpret_cast<float*>(p.o.y)[m * p.o.y_stride + n] = out;
             else reinterpret_cast<__nv_bfloat16*>(p.o.y)[m * p.o.y_stride + n] = __float2bfloat16_rn(out);
         }
+        st = 0;
+        buf ^= 1;
+        tile += gridDim.x;
     };
-    for (int item = 0; item < total; item += 2) {
-        step(item, wa);
-        if (item + 1 < total) step(item + 1, wb);
+    while (tile < tiles) {
+#pragma unroll
+        for (int i = 0; i < I8_TOKEN_AHEAD; ++i)
+            if (tile < tiles) step(w[i]);
     }
 }
 

@@ -161,7 +161,7 @@ int launch_token(const Int8TokenParams& p, bool chained, cudaStream_t stream) {
     constexpr int WIDTH = GATED ? 8 : 8 * CG;
     const int tiles = (p.o.outs + WIDTH - 1) / WIDTH;
     const size_t smem = token_smem(p.o.M, p.o.K);
-    const int resident = 148 * (RG <= 2 && smem <= 96 * 1024 ? 2 : 1);
+    const int resident = 148 * (smem <= 96 * 1024 ? 2 : 1);
     return launch<k_int8_token<RG, CG, GATED, T, VEC>>((unsigned)(tiles < resident ? tiles : resident), 256, smem, I8_TOKEN_SMEM, 1,
                                                        chained, stream, p);
 }
@@ -175,12 +175,12 @@ int token_width(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t
 template <class T, bool VEC>
 int token_rows(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t stream) {
     if (p.o.M <= 8) return token_width<1, T, VEC>(p, gated, chained, stream);
-    if (p.o.M <= 16) return token_width<2, T, VEC>(p, gated, chained, stream);
-    return token_width<4, T, VEC>(p, gated, chained, stream);
+    return token_width<2, T, VEC>(p, gated, chained, stream);
 }
 bool token_takes(const sd_int8_linear_args* a) { return a->rows <= I8_TOKEN_ROWS && token_smem((int)a->rows, a->K) <= I8_TOKEN_SMEM; }
-// Few entries: every CTA quantises the rows for itself, which saves a launch; past that its reading costs more.
-constexpr long long TOKEN_FUSED_ENTRIES = 16384;
+// Few entries: every CTA quantises the rows for itself, which saves a launch; past that it costs more (4 x 1024 entries: 5.9 us
+// against 6.0, 8 x 1024: 7.9 against 6.2).
+constexpr long long TOKEN_FUSED_ENTRIES = 4096;
 bool token_fuses(const sd_int8_linear_args* a) {
     return token_takes(a) && a->x_type == SD_BF16 && aligned(a->x) && a->x_stride % 8 == 0 && a->K % 8 == 0 && a->rows * a->K <= TOKEN_FUSED_ENTRIES;
 }
