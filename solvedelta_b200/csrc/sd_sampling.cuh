@@ -93,20 +93,22 @@ struct SampleShared {
     unsigned ties;
 };
 
-// 2^(44 - (n + r) / 128) to the nearest whole number, 0 <= n < 45 * 128 and |r| little over 1/2: 2^(-n / 128) from a table and
-// an exponent, 2^(-r / 128) from the exponential's series, cut behind the fourth power (the term left out is below 2^-49).
-// Table-driven exponential: P. T. P. Tang, ACM TOMS 15 (1989).
-__device__ __forceinline__ u64 fixed_power(int n, double r, const double* table) {
+// 2^(44 - (n + r) / 128) to the nearest whole number, |r| little over 1/2, and 0 from n = 45 * 128 on: 2^(-n / 128) from a table
+// and an exponent, 2^(-r / 128) from the exponential's series, cut behind the fourth power (the term left out is below 2^-49).
+// Table-driven exponential: P. T. P. Tang, ACM TOMS 15 (1989).  A double holds the whole number, and sums of 512 of them.
+__device__ __forceinline__ double fixed_power(int n, double r, const double* table) {
     constexpr double L = -0.693147180559945309417 / SAMPLE_TABLE;
     double e = fma(r, L * L * L * L / 24, L * L * L / 6);
     e = fma(r, e, L * L / 2);
     e = fma(r, e, L);
     e = fma(r, e, 1.0);
     const double p = table[n & (SAMPLE_TABLE - 1)];
-    const double scaled = __hiloint2double(__double2hiint(p) + ((SAMPLE_WEIGHT_BITS - (n >> 7)) << 20), __double2loint(p));
-    return (u64)__double_as_longlong(fma(e, scaled, 0x1p52)) - (u64)__double_as_longlong(0x1p52);
+    const int high = __double2hiint(p) + ((SAMPLE_WEIGHT_BITS - (n >> 7)) << 20);
+    const double w = fma(e, __hiloint2double(high, __double2loint(p)), 0x1p52) - 0x1p52;   // rounded by the sum
+    return n < SAMPLE_RANGE * SAMPLE_TABLE ? w : 0.0;   // farther entries have no r: they may be infinite
 }
 static_assert(SAMPLE_TABLE == 128, "fixed_power shifts by seven bits");
+static_assert(SAMPLE_MAX_VOCAB / SAMPLE_THREADS <= 512, "a lane's sum of weights is exact");
 
 // Shared memory of CTA `r` of the cluster, at the place of `p` in this one.
 __device__ __forceinline__ unsigned cluster_address(const void* p, int r) {
@@ -178,12 +180,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         }
     };
 
-    bool infinite = false;   // there are infinite logits: they count as zeros, everything else as -infinity
+    // A NaN is never drawn; where there are infinite logits they count as zeros and everything else as -infinity.  Rows have
+    // neither as a rule: `odd` says whether the warp's range needs the second look.
+    bool infinite = false, odd = false;
     const auto clean = [&](T (&e)[VE]) SAMPLE_INLINE {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
             const float f = to_float(e[j]);
-            if (f != f) e[j] = T(-INFINITY);   // a NaN is never drawn
+            if (f != f) e[j] = T(-INFINITY);
             else if (infinite) e[j] = f == INFINITY ? T(0.f) : T(-INFINITY);
         }
     };
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
 #pragma unroll
                     for (int j = 0; j < VE; ++j) e[j] = T(-INFINITY);
                 }
-                clean(e);
+                if (odd) clean(e);
                 f(v, e);
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -234,21 +238,28 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     };
 
     float top = -INFINITY;
+    bool nans = false;
+    const auto look = [&](const T (&e)[VE]) SAMPLE_INLINE {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const float f = to_float(e[j]);
+            nans |= f != f;
+            top = fmaxf(top, f);   // of a number and a NaN: the number
+        }
+    };
     if constexpr (STAGED) {
 #pragma unroll 4
         for (int v = v0 + lane; v < v1; v += 32) {
             alignas(16) T e[VE];
             load(v, e);
-            clean(e);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) top = fmaxf(top, to_float(e[j]));
+            look(e);
             *reinterpret_cast<uint4*>(s_x + v * VE) = *reinterpret_cast<const uint4*>(e);
         }
+        if (nans)   // a lane's own vectors
+            for (int v = v0 + lane; v < v1; v += 32) clean(*reinterpret_cast<T(*)[VE]>(s_x + v * VE));
     } else {
-        scan_range([&](int, const T (&e)[VE]) {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) top = fmaxf(top, to_float(e[j]));
-        });
+        scan_range([&](int, const T (&e)[VE]) { look(e); });
+        odd = __any_sync(0xffffffffu, nans);
     }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
@@ -272,7 +283,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         return;
     }
     if (top == INFINITY) {
-        infinite = true;
+        infinite = odd = true;
         top = 0.f;
         if constexpr (STAGED) {
             for (int v = v0 + lane; v < v1; v += 32) clean(*reinterpret_cast<T(*)[VE]>(s_x + v * VE));
@@ -299,12 +310,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         // a sum with 1.5 * 2^23 is rounded to a whole number
         return __float_as_int(fmaf(fminf(top - v, far), slope_f, 12582912.f)) - __float_as_int(12582912.f);
     };
-    const auto weight_at = [&](float v, int n) SAMPLE_INLINE -> u64 {
+    const auto weight_at = [&](float v, int n) SAMPLE_INLINE {
         const double whole = __hiloint2double(0x43380000, n) - 6755399441055744.0;   // 1.5 * 2^52 + n, less that
-        const u64 w = fixed_power(n, fma((double)top - (double)v, slope, -whole), sh.power);
-        return n < SAMPLE_RANGE * SAMPLE_TABLE ? w : 0ull;
+        return fixed_power(n, fma((double)top - (double)v, slope, -whole), sh.power);
     };
-    const auto weight = [&](float v) SAMPLE_INLINE -> u64 { return weight_at(v, whole_steps(v)); };
+    const auto weight_of = [&](float v) SAMPLE_INLINE { return weight_at(v, whole_steps(v)); };
+    const auto weight = [&](float v) SAMPLE_INLINE { return (u64)weight_of(v); };
     const auto bin_of = [&](float v) SAMPLE_INLINE { return whole_steps(v) >> SAMPLE_BIN_BITS; };
 
     float cut = -INFINITY;   // entries under it were dropped
@@ -546,25 +557,30 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         const double clipped = u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0;   // a NaN counts as zero
         return __umul64hi(all, (u64)(clipped * 0x1p64));
     };
-    // The threads' keys in descending order, over as many threads as `n` needs (a power of two), zeros behind: a bitonic
-    // network, inside a warp by shuffles and between warps through `scratch`.
+    // The first `n` threads' keys in descending order, zeros behind, through `scratch`.  Every key is compared with every other
+    // one, by as many threads as there are for it: two barriers where a sorting network takes two for every step between
+    // warps (132 keys: 9000 clocks in one).
     const auto sort_down = [&](auto key, unsigned n, auto* scratch) SAMPLE_INLINE {
-        const int size_all = n > 1 ? 1 << (32 - __clz((int)n - 1)) : 1;
-        const bool active = warp * 32 < size_all;
-        for (int size = 2; size <= size_all; size <<= 1)
-            for (int j = size >> 1; j > 0; j >>= 1) {
-                auto other = key;
-                if (j >= 32) {
-                    __syncthreads();
-                    if (active) scratch[tid] = key;
-                    __syncthreads();
-                    if (active) other = scratch[tid ^ j];
-                } else if (active) {
-                    other = __shfl_xor_sync(0xffffffffu, key, j);
-                }
-                const bool larger = ((tid & size) == 0) == ((tid & j) == 0);
-                if (larger ? other > key : other < key) key = other;
+        __syncthreads();
+        if (tid < n) scratch[tid] = key;
+        __syncthreads();
+        const int parts_log2 = min(5, 31 - __clz((int)(SAMPLE_THREADS / n))), parts = 1 << parts_log2;
+        const unsigned i = (unsigned)tid >> parts_log2;
+        decltype(key) mine_of = 0;
+        unsigned above = 0;
+        if (i < n) {
+            mine_of = scratch[i];
+#pragma unroll 4
+            for (unsigned j = tid & (parts - 1); j < n; j += parts) {
+                const auto other = scratch[j];
+                above += other > mine_of || (other == mine_of && j < i) ? 1u : 0u;
             }
+        }
+        for (int s = 1; s < parts; s <<= 1) above += __shfl_xor_sync(0xffffffffu, above, s);
+        __syncthreads();
+        if (i < n && (tid & (parts - 1)) == 0) scratch[above] = mine_of;
+        __syncthreads();
+        key = tid < n ? scratch[tid] : 0;
         return key;
     };
     // The rest of the row's work where few candidates are left, by the first CTA: one a thread, sorted by logit and place.
@@ -601,17 +617,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     // `before` is that sum over the bins in front; with `sum_front` it is added up here.
     // False: the border is in front of the step.
     const auto refine = [&](int step, bool by_mass, unsigned count, double target, u64 before, bool sum_front) SAMPLE_INLINE {
-        u64 front = 0;
+        double front = 0.0;
         unsigned n = 0;
         each([&](float v) {
             const int b = bin_of(v);
             if (b == step) n += v > -INFINITY && !(v < edge);
-            else if (sum_front && b < step) front += weight(v);
+            else if (sum_front && b < step) front += weight_of(v);
         });
         n = __reduce_add_sync(0xffffffffu, n);
         if (lane == 0) sh.warp_eq[warp] = n;
-        if (sum_front) block_sum(front);
-        else __syncthreads();
+        if (sum_front) block_sum((u64)front);
         unsigned in_warps = lane < SAMPLE_WARPS ? sh.warp_eq[lane] : 0;
         const unsigned before_warp = __reduce_add_sync(0xffffffffu, lane < warp ? in_warps : 0);
         in_warps = __reduce_add_sync(0xffffffffu, in_warps);
@@ -768,19 +783,22 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         else if (step >= 0) rule = TOP_K;
         if (by_p && rule == DONE) rule = TOP_P_LEFT;
     } else if (by_p) {
-        // the sum of all weights, and a histogram of their upper 16 bits (relative to the largest of the bin): its running
-        // sums are not above the true ones, so the border is not behind the bin in which they reach the target
+        // the sum of all weights, and a histogram of their upper 16 bits (against 2^(43 - a), the binade of the bin): its
+        // running sums are not above the true ones, so the border is not behind the bin in which they reach the target
         constexpr int PER_BINADE = SAMPLE_TABLE >> SAMPLE_BIN_BITS;
-        const auto bin_shift = [](int b) { return max(0, SAMPLE_WEIGHT_BITS - 15 - b / PER_BINADE); };
-        u64 sum = 0;
+        double sum = 0.0;
         each_loaded([&](float v) {
-            const int n = whole_steps(v), b = n >> SAMPLE_BIN_BITS;
-            const u64 w = weight_at(v, n);
+            const int n = whole_steps(v);
+            const double w = weight_at(v, n);
             sum += w;
-            if (w != 0) atomicAdd(&sh.count[b], (unsigned)(w >> bin_shift(b)));
+            const int high = __double2hiint(w), binades = (high >> 20) - (1023 + 43) + (n >> 7);   // over 2^(43 - a): 0, or 1 at its end
+            if (high != 0) atomicAdd(&sh.count[n >> SAMPLE_BIN_BITS], (unsigned)((high & 0xfffff) | 0x100000) << (binades + 1) >> 6);
         });
-        block_sum(sum);
-        for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.mass[b] = (u64)sh.count[b] << bin_shift(b);
+        block_sum((u64)sum);
+        for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
+            const int up = SAMPLE_WEIGHT_BITS - 1 - 15 - b / PER_BINADE;
+            sh.mass[b] = up >= 0 ? (u64)sh.count[b] << up : (u64)sh.count[b] >> -up;
+        }
         publish(false, true);
         u64 all = 0;
         for (int r = 0; r < C; ++r) all += read(&sh.total_gt, r);
@@ -800,9 +818,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     while (rule != DONE) {
         if (rule == TOP_P_LEFT) {
             if (by_k) {   // the weight of what top-k keeps
-                u64 sum = 0;
-                each([&](float v) { if (v > edge) sum += weight(v); });
-                block_sum(sum);
+                double sum = 0.0;
+                each([&](float v) { if (v > edge) sum += weight_of(v); });
+                block_sum((u64)sum);
                 everywhere();
                 u64 all = edge > -INFINITY ? ties * weight(edge) : 0ull;
                 for (int r = 0; r < C; ++r) all += read(&sh.total_gt, r);
@@ -830,19 +848,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         return reach == INFINITY || steps_below(v) <= reach ? weight(v) : 0ull;
     };
     const u64 edge_weight = edge > -INFINITY ? drawn_weight(edge) : 0ull;
-    u64 gt = 0;
+    double gt_sum = 0.0;
     unsigned eq = 0;
     if (cut == -INFINITY) {   // no rule: no border either
-        each_loaded([&](float v) { gt += weight(v); });
+        each_loaded([&](float v) { gt_sum += weight_of(v); });
     } else {
         each([&](float v) {
-            if (v > edge) gt += drawn_weight(v);
+            if (v > edge) gt_sum += reach == INFINITY || steps_below(v) <= reach ? weight_of(v) : 0.0;
             else if (v == edge) ++eq;
         });
     }
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) sh.warp_eq[warp] = eq;
-    block_sum(gt);
+    block_sum((u64)gt_sum);
     if (tid == 0) {
         unsigned b = 0;
         for (int w = 0; w < SAMPLE_WARPS; ++w) b += sh.warp_eq[w];
