@@ -576,7 +576,7 @@ typedef struct {
     const void *logits;            /* [rows][V], rows stride elements apart */
     int64_t stride;
     const float *uniform;          /* [rows] */
-    /* one value per row, or NULL: the number below for all */
+    /* one value per row, or NULL: the number below for all, rounded to FP32 like those */
     const float *temperature_row;
     const int32_t *top_k_row;
     const float *top_p_row;

@@ -627,6 +627,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         n = __reduce_add_sync(0xffffffffu, n);
         if (lane == 0) sh.warp_eq[warp] = n;
         if (sum_front) block_sum((u64)front);
+        else __syncthreads();
         unsigned in_warps = lane < SAMPLE_WARPS ? sh.warp_eq[lane] : 0;
         const unsigned before_warp = __reduce_add_sync(0xffffffffu, lane < warp ? in_warps : 0);
         in_warps = __reduce_add_sync(0xffffffffu, in_warps);

@@ -288,7 +288,8 @@ int sd_sample_tokens(const sd_sample_tokens_args* a, void* stream_) {
     p.V = a->V;
     p.logits = a->logits; p.stride = a->stride; p.uniform = a->uniform;
     p.temperature_row = a->temperature_row; p.top_k_row = a->top_k_row; p.top_p_row = a->top_p_row; p.min_p_row = a->min_p_row;
-    p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
+    // a number counts as its FP32 value, as in a tensor of settings: both give the same tokens
+    p.temperature = (float)a->temperature; p.top_p = (float)a->top_p; p.min_p = (float)a->min_p; p.top_k = a->top_k;
     p.empty_token = a->empty_token;
     p.tokens = reinterpret_cast<long long*>(a->tokens);
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);

@@ -19,8 +19,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: U
     ``top_k`` keeps the first k of them (0: all), ``top_p`` of those the ones before which less than ``top_p`` of their
     weight lies (1: all; the first always stays), ``min_p`` those whose weight is at least ``min_p`` times the largest.
     The token is the first index at which the running sum of the kept weights, in the order of the vocabulary, exceeds
-    ``uniform`` times their sum.  ``temperature`` 0 takes the first of the order.  Each setting is a number or a tensor
-    ``[B]`` on the device of the logits, one value for each row (numbers out of range are refused; in a tensor a
+    ``uniform`` times their sum.  ``temperature`` 0 takes the first of the order.  Each setting is a number (taken in
+    FP32) or a tensor ``[B]`` on the device of the logits, one value for each row (numbers out of range are refused; in a tensor a
     temperature that is not above 1e-30 and a ``top_p`` that is not above 0 take the first of the order, a ``top_k``
     below 1, a ``top_p`` above 1 and a ``min_p`` below 0 keep all, a ``min_p`` above 1 counts as 1).  A
     temperature above 1e30 counts as 1e30.

@@ -72,5 +72,7 @@ def token(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, empty=-1):
 
 def tokens(logits, uniform, **settings):
     x, u = as64(logits), as64(uniform)
-    rows = {k: (v.detach().cpu().tolist() if torch.is_tensor(v) else [v] * len(x)) for k, v in settings.items()}
+    # settings are FP32 numbers, whether one for all rows or a tensor
+    rows = {k: (v.detach().cpu().tolist() if torch.is_tensor(v) else [v if k == "top_k" else float(np.float32(v))] * len(x))
+            for k, v in settings.items()}
     return [token(x[i], u[i], **{k: v[i] for k, v in rows.items()}) for i in range(len(x))]

@@ -50,6 +50,26 @@ def test_rows_too_long_for_shared_memory(dtype, rows, vocab):
         _same(logits, u, **settings)
 
 
+@pytest.mark.parametrize("dtype,rows,vocab", ((torch.float32, 30, 30000), (torch.bfloat16, 140, 30000), (torch.float32, 400, 20000),
+                                              (torch.float32, 300, 40000), (torch.bfloat16, 200, 60000), (torch.float32, 2, 262144)))
+def test_borders_among_thousands_of_candidates(dtype, rows, vocab):
+    """More candidates than the first CTA lists, borders of both rules: the definition's tokens, and the same ones every time."""
+    logits, u = _logits(rows, vocab, 21, dtype)
+    for settings in (dict(top_k=600), dict(top_k=2000, temperature=1.4), dict(top_k=5000, top_p=0.97), dict(top_p=0.95, temperature=0.7),
+                     dict(top_p=0.99, temperature=2.0), dict(top_k=4000, min_p=1e-3)):
+        _same(logits, u, **settings)
+        first = sd.sample_tokens(logits, u, **settings)
+        for _ in range(12):
+            assert torch.equal(sd.sample_tokens(logits, u, **settings), first)
+
+
+def test_a_number_and_a_tensor_of_it_draw_the_same():
+    logits, u = _logits(50, 9000, 4)
+    for name, value in (("temperature", 0.7), ("top_p", 0.95), ("min_p", 0.01), ("top_k", 700)):
+        full = torch.full((50,), value, device="cuda", dtype=torch.int32 if name == "top_k" else torch.float32)
+        assert torch.equal(sd.sample_tokens(logits, u, **{name: value}), sd.sample_tokens(logits, u, **{name: full}))
+
+
 def test_settings_of_each_row():
     logits, u = _logits(64, 3000, 3)
     gen = torch.Generator().manual_seed(1)
