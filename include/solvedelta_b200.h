@@ -398,7 +398,9 @@ int sd_backward_launches(const sd_shape *shape);
  * contraction of a step (X = P + Q St) never completed, 2 = the second (state update),
  * 3 = a step's Q panel never landed, 4 = its R / P panels never landed, 5 = the slot of
  * the R / P panels was never released; codes 6-7 from the tensor-memory output contraction:
- * 6 = its panels never landed, 7 = the contraction never completed.  No upstream counterpart.
+ * 6 = its panels never landed, 7 = the contraction never completed; codes 9-11 from the 8-bit products: 9 = a stage of
+ * the ring was never released, 10 = a stage never landed or an accumulator was never emptied, 11 = an accumulator never
+ * completed.  No upstream counterpart.
  *
  * sd_device_fault waits for the device and returns the word (0 = no fault, -1 = the device
  * could not be read); the word stays set until sd_device_fault_clear() (which also waits

@@ -90,7 +90,7 @@ Tensor product(const Tensor& x, const Tensor& scale_in, const Tensor& weight_in,
     const int64_t N = weight_in.size(0), K = weight_in.size(1);
     value_error(x.dim() < 1 || x.size(-1) != K, "the last axis of the rows must be as long as the weight's");
     check_width(K);
-    value_error(N < 1 || N > 0x7fffffffLL, "weight must have at least one row");
+    value_error(N < 1 || N > 0x7fffff00LL, "weight must have at least one row, and fewer than 2^31");
     value_error(swiglu && N % 2 != 0, "with swiglu the weight holds gate rows and as many value rows");
     type_error(weight_scale_in.scalar_type() != at::kFloat, "weight_scale must be FP32");
     value_error(!is_shape(weight_scale_in, {N}), "weight_scale must be [N]");

@@ -208,7 +208,8 @@ int launch_sample(SampleParams p, long long rows, cudaStream_t stream) {
 template <class T>
 int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
     // as many CTAs a row as the SMs take at once, two on each, with 2048 entries at least; and so many that the rows in work
-    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32: 376 us with one CTA, TODO with two)
+    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32, top-p: 552 us with one CTA a row, 398 with
+    // two, 492 with four)
     const auto worth = [&](int c) {
         return p.V >= c * 2048 && (rows * c <= 2 * 148 || 2 * 148 / (c / 2) * (long long)p.V * (int)sizeof(T) > SAMPLE_L2);
     };
@@ -243,7 +244,7 @@ int sd_int8_linear(const sd_int8_linear_args* a, void* stream_) {
     if (!aligned(a->weight) || a->weight_stride % 16 != 0 || a->weight_stride < padded(a->K) ||
         (a->x_type == SD_I8 && (!aligned(a->x) || a->x_stride % 16 != 0 || (a->rows > 1 && a->x_stride < padded(a->K)))))
         return SD_ERR_INVALID_ARGUMENT;
-    if (a->K > MAX_K || a->rows > 0x7fffff00LL) return SD_ERR_UNSUPPORTED_SHAPE;
+    if (a->K > MAX_K || a->rows > 0x7fffff00LL || a->N > 0x7fffff00) return SD_ERR_UNSUPPORTED_SHAPE;   // rounded up to tiles, both stay in 32 bits
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     Int8Params p{};
     p.M = (int)a->rows; p.outs = a->swiglu ? a->N / 2 : a->N; p.K = a->K;

@@ -17,7 +17,7 @@ from . import _lib
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of the rows of ``x`` ``[..., K]`` (BF16 or FP32 CUDA): ``q`` int8 ``[..., K]``, its rows padded to
     whole groups of 16 bytes, ``scale`` FP32 ``[...]``.  A row of zeros has scale 0; a row with an infinity or a NaN has
-    ``q = 0`` and scale NaN, so that everything computed from it is NaN."""
+    ``q = 0`` and scale NaN, so that everything computed from it is NaN.  Neither output carries a gradient."""
     return _lib.host().quantize_rows(x)
 
 

@@ -437,7 +437,8 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
     def quantize_int8(self, head: bool = False) -> "SolveDeltaForCausalLM":
         """Hold the gated MLPs' weights, and with ``head`` the vocabulary projection's, in int8 (:class:`Int8Linear`), for
         inference on a CUDA device: half of their bytes in a cached token, twice the tensor rate in a prompt.  The mixers
-        stay in BF16.  In place, not reversible; quantised modules are left as they are.  Returns the model."""
+        stay in BF16.  In place, not reversible; quantised modules are left as they are.  Checkpoints are those of the model
+        before: quantise after loading.  Returns the model."""
         if head and self.config.tie_word_embeddings:
             raise ValueError("a tied head shares the embedding's weight and cannot be quantised")
         for layer in self.model.layers:

@@ -60,6 +60,7 @@ def test_argument_errors_are_status_codes(lib):
     assert [linear(weight_stride=96), linear(weight=at + 4), linear(x_stride=100), linear(x=at + 1), linear(x_scale=None),
             linear(y_type=_lib.I8), linear(x_type=7), linear(N=7, swiglu=1), linear(K=0), linear(bias=at, bias_type=_lib.I8)] == [-1] * 10
     assert linear(K=131073, weight_stride=131088, x_stride=131088) == -2
+    assert linear(N=0x7fffff01) == -2 and linear(rows=0x7fffff01) == -2
     assert linear(x_type=_lib.BF16, x_stride=100) == -3   # no room for the quantised rows
 
     def scratch(count, width, x_type):
