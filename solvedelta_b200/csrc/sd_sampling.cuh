@@ -66,9 +66,9 @@ typedef unsigned long long u64;
 // the kernel's parts share its variables by reference: one that is not inlined would keep them in local memory
 #define SAMPLE_INLINE __attribute__((always_inline))
 
-// Order-preserving bits of a float, and back.
+// Order-preserving bits of a float (both zeros have the same), and back.
 __device__ __forceinline__ unsigned order_bits(float x) {
-    const unsigned b = __float_as_uint(x);
+    const unsigned b = __float_as_uint(__fadd_rn(x, 0.f));
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float from_order_bits(unsigned k) {

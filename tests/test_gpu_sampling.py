@@ -106,6 +106,16 @@ def test_equal_logits_go_by_index():
     assert sd.sample_tokens(flat[:2], torch.tensor([0.5, 0.999], device="cuda"), top_k=2).tolist() == [1, 1]
 
 
+def test_both_zeros_are_equal():
+    for dtype, vocab in itertools.product((torch.bfloat16, torch.float32), (40, 3000, 30000)):
+        logits = torch.zeros(8, vocab, dtype=dtype, device="cuda")
+        logits[:, ::2] = -0.0
+        logits[:, -1] = 1.0
+        u = torch.tensor([0.0, 0.1, 0.25, 0.5, 0.625, 0.75, 0.9, 0.99], device="cuda")
+        for settings in (dict(), dict(top_k=3), dict(top_k=11), dict(top_k=vocab // 2), dict(top_p=0.3), dict(top_p=0.5, top_k=vocab - 3), dict(temperature=0.0)):
+            _same(logits, u, **settings)
+
+
 def test_borders_of_the_uniform_number():
     logits, _ = _logits(6, 5000, 8)
     u = torch.tensor([0.0, 2.0 ** -24, 1 - 2.0 ** -24, 0.5, 1e-30, 0.999], device="cuda")
