@@ -64,7 +64,8 @@ int quantize_launch(const QuantizeParams& p, bool chained, cudaStream_t stream) 
 }
 template <class T, bool VEC, int H>
 int quantize_width(const QuantizeParams& p, bool chained, cudaStream_t stream) {
-    // as few warps a row as hold it in registers, but more while the SMs are not full of warps (2048 rows: 32 each)
+    // as few warps a row as hold it in registers (16384 x 2048: 28 us with one, 38 with eight), but more while the SMs are not full
+    // of warps (64 x 1024: 1.9 us with eight, 2.9 with one)
     const auto enough = [&](int w) { return (long long)w * 256 * H >= p.K && p.rows * w >= 148 * 16; };
     if (enough(1)) return quantize_launch<T, VEC, 1, H>(p, chained, stream);
     if (enough(2)) return quantize_launch<T, VEC, 2, H>(p, chained, stream);
@@ -114,7 +115,8 @@ int launch_matmul(Int8Params p, const sd_int8_linear_args* a, const void* q, lon
     return launch<k_int8_matmul<BN, GATED, F32, PAIR>>(workers * CTAS, I8_THREADS, Int8Tile<BN, PAIR>::SMEM, Int8Tile<BN, PAIR>::SMEM, CTAS,
                                                        chained, stream, p, x_map, w_map, fault);
 }
-// How many CTAs share a tile of 128 x 64 (as a power of two): as many as the SMs have room for, four steps of K each at least.
+// How many CTAs share a tile of 128 x 64 (as a power of two): as many as the SMs have room for, four steps of K each at least
+// (64 x 5632 x 2048: 8.7 us with four, 16.2 with one; 128 x 2816 x 1024: 7.5 and 9.9).
 int split_log2(long long tiles, int K) {
     const int blocks = (K + I8_BK - 1) / I8_BK;
     int n = 0;
@@ -141,8 +143,10 @@ int matmul_tile(const Int8Params& p, const sd_int8_linear_args* a, const void* q
         const int outs = GATED ? bn / 2 : bn;
         return (long long)((p.M + bm - 1) / bm) * ((p.outs + outs - 1) / outs);
     };
-    // the widest tile that still gives every SM one
-    if (tiles(256, 256) >= 74 && p.M > 128) return launch_matmul<256, GATED, F32, true>(p, a, q, q_stride, chained, stream);
+    // Pairs of CTAs from half of the SMs on (700 x 2048 x 4096, 48 tiles: 11.3 us, tiles of one CTA 14.9; 300 x 2048 x 2048, 16
+    // tiles: 10.9 against 8.5); else the wider tile while it gives every SM one (2048 x 1024 x 2816: 128 columns 13.5 us, 64 18.2;
+    // 128 x 1024 x 5632, 44 tiles of 128 columns: 6.4 against 5.9).
+    if (tiles(256, 256) >= 37 && p.M > 128) return launch_matmul<256, GATED, F32, true>(p, a, q, q_stride, chained, stream);
     if (tiles(128, 128) >= 148) return launch_matmul<128, GATED, F32, false>(p, a, q, q_stride, chained, stream);
     const int ctas_log2 = split_log2(tiles(128, 64), p.K);
     if (ctas_log2 > 0) return launch_split<GATED, F32>(p, a, q, q_stride, ctas_log2, chained, stream);
@@ -168,8 +172,9 @@ int launch_token(const Int8TokenParams& p, bool chained, cudaStream_t stream) {
 template <int RG, class T, bool VEC>
 int token_width(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t stream) {
     if (gated) return launch_token<RG, 2, true, T, VEC>(p, chained, stream);
-    // 16 columns a tile while that gives every SM one, else 8
-    return p.o.outs >= 16 * 148 ? launch_token<RG, 2, false, T, VEC>(p, chained, stream)
+    // 16 columns a tile while that keeps most SMs busy (one row, 1024 x 2048: 2.9 us, with 8 columns 3.1; 2048 x 4096: 4.3 and 4.8),
+    // else 8 (2816 x 1024: 3.2 us, with 16 columns 3.7)
+    return p.o.outs >= 16 * 128 ? launch_token<RG, 2, false, T, VEC>(p, chained, stream)
                                 : launch_token<RG, 1, false, T, VEC>(p, chained, stream);
 }
 template <class T, bool VEC>
