@@ -19,7 +19,10 @@
 // * up to 512 candidates go to the first CTA, one a thread, which sorts them, sums them up and draws;
 // * more are moved together by their warps.  The exact border comes from the entries of its step, gathered, or, where those
 //   are more than 512, from further histograms over equal steps of the logit's bits, until one value is left; sums and draw
-//   go over what was moved.
+//   go over what was moved;
+// * where that is too much for shared memory, the entries of the border's step alone are moved, and the weights in front of it
+//   are summed up once (512 rows of 128000, FP32, N(0, 4), top-p 0.95, 30000 kept of each: 1026 us when every histogram read
+//   the row again, 623 so).
 //
 // What bounds it.  One row of 32000 (top-k 50 and top-p: 10 us): a dozen phases of 0.3 to 2 us each, cluster barriers and reads
 // of another CTA's memory.  512 rows of 128000 in FP32 (top-p 0.95: 375 us; their 262 MB take 40 us): instructions, some 140
@@ -195,7 +198,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             else if (infinite) e[j] = f == INFINITY ? T(0.f) : T(-INFINITY);
         }
     };
-    // The vectors of the warp's range, 32 at a time: f(v, entries), all lanes together (v past the range: -infinity).
+    // The vectors of the warp's range, 32 at a time: f(v, entries), all lanes together (v past the range: -infinity), as long as
+    // it returns true in all of them.
     const auto scan_range = [&](auto&& f) SAMPLE_INLINE {
         alignas(16) T e[VE];
         if constexpr (STAGED) {
@@ -207,7 +211,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
 #pragma unroll
                     for (int j = 0; j < VE; ++j) e[j] = T(-INFINITY);
                 }
-                f(v, e);
+                if (!f(v, e)) break;
             }
         } else {
             const auto inside = [&](int v) SAMPLE_INLINE { return first + v * VE - shift >= 0 && first + v * VE - shift + VE <= p.V; };
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                     for (int j = 0; j < VE; ++j) e[j] = T(-INFINITY);
                 }
                 if (odd) clean(e);
-                f(v, e);
+                if (!f(v, e)) break;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         if (nans)   // a lane's own vectors
             for (int v = v0 + lane; v < v1; v += 32) clean(*reinterpret_cast<T(*)[VE]>(s_x + v * VE));
     } else {
-        scan_range([&](int, const T (&e)[VE]) { look(e); });
+        scan_range([&](int, const T (&e)[VE]) SAMPLE_INLINE { look(e); return true; });
         odd = __any_sync(0xffffffffu, nans);
     }
 #pragma unroll
@@ -328,6 +332,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         scan_range([&](int, const T (&e)[VE]) {
 #pragma unroll
             for (int j = 0; j < VE; ++j) f(to_float(e[j]));
+            return true;
         });
     };
     // Every entry that is left.
@@ -467,17 +472,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         all = __shfl_sync(0xffffffffu, upto, 31);
         return upto - n;
     };
-    // Walks over the warp's range: f(vector, its entries that stay, how many of them are in front of the vector's).
-    const auto walk = [&](auto&& f) SAMPLE_INLINE {
+    // Walks over the warp's range until more than `most` entries have stayed, which it counts: f(vector, its entries that stay,
+    // how many of them are in front of the vector's).
+    const auto walk = [&](int most, auto&& f) SAMPLE_INLINE {
         int kept = 0;
         scan_range([&](int v, const T (&e)[VE]) {
             const unsigned stays = in_front(e);
-            if (!__any_sync(0xffffffffu, stays)) return;
+            if (!__any_sync(0xffffffffu, stays)) return true;
             int all;
             const int at = kept + prefix(__popc(stays), all);
             f(v, e, stays, at);
             kept += all;
             __syncwarp();
+            return kept <= most;
         });
         return kept;
     };
@@ -489,10 +496,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         cut = end_of_bin(bin);
         int n = 0;
         if constexpr (STAGED) {
-            scan_range([&](int, const T (&e)[VE]) { n += __popc(in_front(e)); });
+            scan_range([&](int, const T (&e)[VE]) { n += __popc(in_front(e)); return true; });
             n = __reduce_add_sync(0xffffffffu, n);
         } else {
-            n = walk([&](int v, const T (&e)[VE], unsigned stays, int at) {
+            n = walk(p.list, [&](int v, const T (&e)[VE], unsigned stays, int at) {
 #pragma unroll
                 for (int j = 0; j < VE; ++j)
                     if (stays >> j & 1) {
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                         ++at;
                     }
             });
-            here = n <= p.list;   // else the range stays where it is
+            here = n <= p.list;   // else the range stays where it is, and there are more than go to the first CTA
             held = n;
         }
         if (lane == 0) sh.warp_eq[warp] = n;
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             write(&sh.count[place], 0, (unsigned)index);
         };
         if constexpr (STAGED) {
-            held = walk([&](int v, const T (&e)[VE], unsigned stays, int at) {
+            held = walk(n, [&](int v, const T (&e)[VE], unsigned stays, int at) {
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < VE; ++j)
@@ -616,19 +623,52 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     // what stays: logits above `edge`, and the first `ties` of those on it
     float edge = -INFINITY;
     unsigned ties = 0;
+    // what refine() leaves for the draw: the lane's sum of the weights in front of the border's step, and the step's entries in
+    // the warp's range where it is read again (-1: not all of them fitted into the list)
+    double front = 0.0;
+    bool fronted = false;
+    int stepped = -1;
 
+    const auto each_in_step = [&](auto&& f) SAMPLE_INLINE {   // of the step at least: in the list, where that holds it
+        if (!here && stepped < 0) {
+            each_loaded(f);
+            return;
+        }
+        const int n = here ? held : stepped;
+        for (int i = lane; i < n; i += 32) f(to_float(mine[i]));
+    };
     // The border inside the bin `step`, on the edge of what a running sum reaches: of weights, `target`; of counts, `count`.
     // `before` is that sum over the bins in front; with `sum_front` it is added up here.
     // False: the border is in front of the step.
     const auto refine = [&](int step, bool by_mass, unsigned count, double target, u64 before, bool sum_front) SAMPLE_INLINE {
-        double front = 0.0;
         unsigned n = 0;
-        each([&](float v) {
-            const int b = bin_of(v);
-            if (b == step) n += v > -INFINITY && !(v < edge);
-            else if (sum_front && b < step) front += weight_of(v);
-        });
-        n = __reduce_add_sync(0xffffffffu, n);
+        front = 0.0;
+        fronted = sum_front;
+        if (STAGED || here) {
+            for (int i = lane; i < held; i += 32) {
+                const float v = to_float(mine[i]);
+                const int b = bin_of(v);
+                if (b == step) n += v > -INFINITY && !(v < edge);
+                else if (sum_front && b < step) front += weight_of(v);
+            }
+            n = __reduce_add_sync(0xffffffffu, n);
+        } else {   // nothing under the cut is in the step or in front of it
+            scan_range([&](int, const T (&e)[VE]) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    const float v = to_float(e[j]);
+                    const int b = bin_of(v);
+                    const bool in = b == step && v > -INFINITY && !(v < edge);
+                    if (sum_front && b < step) front += weight_of(v);
+                    const unsigned lanes = __ballot_sync(0xffffffffu, in);
+                    const unsigned at = n + __popc(lanes & ((1u << lane) - 1));
+                    if (in && at < p.list) mine[at] = e[j];
+                    n += __popc(lanes);
+                }
+                return true;
+            });
+            stepped = n <= p.list ? (int)n : -1;
+        }
         if (lane == 0) sh.warp_eq[warp] = n;
         if (sum_front) block_sum((u64)front);
         else __syncthreads();
@@ -649,15 +689,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         if (all <= SAMPLE_THREADS) {
             // every CTA gets all entries of the step and sorts them
             unsigned at = before_slice + before_warp;
-            for (int i0 = 0; i0 < (here ? held : 0); i0 += 32) {
-                const float v = i0 + lane < held ? to_float(mine[i0 + lane]) : -INFINITY;
+            const int on_hand = here ? held : stepped;
+            for (int i0 = 0; i0 < on_hand; i0 += 32) {
+                const float v = i0 + lane < on_hand ? to_float(mine[i0 + lane]) : -INFINITY;
                 const bool in = v > -INFINITY && !(v < edge) && bin_of(v) == step;
                 const unsigned lanes = __ballot_sync(0xffffffffu, in);
                 if (in)
                     for (int r = 0; r < C; ++r) write(&sh.count[at + __popc(lanes & ((1u << lane) - 1))], r, order_bits(v));
                 at += __popc(lanes);
             }
-            if (!here)
+            if (on_hand < 0)
                 scan_range([&](int, const T (&e)[VE]) {
 #pragma unroll
                     for (int j = 0; j < VE; ++j) {
@@ -668,6 +709,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                             for (int r = 0; r < C; ++r) write(&sh.count[at + __popc(lanes & ((1u << lane) - 1))], r, order_bits(v));
                         at += __popc(lanes);
                     }
+                    return true;
                 });
             everywhere();
             const unsigned key = sort_down(tid < all ? sh.count[tid] : 0u, all, sh.count);
@@ -689,7 +731,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             return true;
         }
         unsigned low = 0xffffffffu, high = 0;
-        each([&](float v) {
+        each_in_step([&](float v) {
             if (bin_of(v) != step || !(v > -INFINITY) || v < edge) return;
             const unsigned k = order_bits(v);
             low = min(low, k);
@@ -718,7 +760,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             const int width = 32 - __clz(high - low), down = width > 10 ? width - 10 : 0;   // 1024 bins
             const u64 carried = sh.before;
             clear();
-            each([&](float v) {
+            each_in_step([&](float v) {
                 const unsigned k = order_bits(v);
                 if (k < low || k > high) return;
                 const int b = (int)((high - k) >> down);
@@ -758,6 +800,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
 #pragma unroll
             for (int j = VE - 1; j >= 0; --j)
                 if (to_float(e[j]) == top) at = min(at, (unsigned)(first + v * VE + j - shift));
+            return true;
         });
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) sh.warp_eq[warp] = at;
@@ -857,7 +900,22 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     unsigned eq = 0;
     if (cut == -INFINITY) {   // no rule: no border either
         each_loaded([&](float v) { gt_sum += weight_of(v); });
+    } else if (fronted && reach == INFINITY) {
+        // every entry in front of the step stays, none behind it
+        if (!here && stepped >= 0) {
+            for (int i = lane; i < stepped; i += 32) {
+                const float v = to_float(mine[i]);
+                if (v > edge) gt_sum += weight_of(v);
+                else if (v == edge) ++eq;
+            }
+        } else {
+            each([&](float v) {
+                if (v == edge) ++eq;
+                else if (v > edge && bin_of(v) == step) gt_sum += weight_of(v);
+            });
+        }
     } else {
+        front = 0.0;
         each([&](float v) {
             if (v > edge) gt_sum += reach == INFINITY || steps_below(v) <= reach ? weight_of(v) : 0.0;
             else if (v == edge) ++eq;
@@ -865,7 +923,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     }
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) sh.warp_eq[warp] = eq;
-    block_sum((u64)gt_sum);
+    block_sum((u64)front + (u64)gt_sum);
     if (tid == 0) {
         unsigned b = 0;
         for (int w = 0; w < SAMPLE_WARPS; ++w) b += sh.warp_eq[w];
@@ -896,9 +954,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     own = sh.warp_sum[warp] + (seen < ties ? min(sh.warp_eq[warp], ties - seen) : 0) * edge_weight;
     if (drawn < before || drawn >= before + own) return;   // another warp's
     if (!here) {   // over the range itself, a vector a lane
-        bool done = false;
         scan_range([&](int v, const T (&e)[VE]) {
-            if (done) return;
             u64 sum = 0;
             int on = 0;
             const unsigned stays = in_front(e);
@@ -935,7 +991,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
             seen += on_all;
-            done = drawn < before;
+            return drawn >= before;
         });
         return;
     }
