@@ -214,30 +214,31 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                 if (!f(v, e)) break;
             }
         } else {
-            const auto inside = [&](int v) SAMPLE_INLINE { return first + v * VE - shift >= 0 && first + v * VE - shift + VE <= p.V; };
-            const auto request = [&](int base) SAMPLE_INLINE {
-                const int v = base + lane;
-                if (v < v1 && inside(v)) {
-                    const unsigned to = tc_smem(ring + (base / 32 % SAMPLE_RING) * 512);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(x + first + v * VE - shift) : "memory");
-                }
+            // only the row's first and last vector may reach outside it
+            const int in0 = v0 + (first + v0 * VE < shift ? 1 : 0);
+            const unsigned in_row = max(0, min(v1, (p.V + shift - first) / VE) - in0);
+            const T* from = x + first + (v0 + lane) * VE - shift;
+            unsigned slot = 0;
+            const auto request = [&](int v, unsigned to) SAMPLE_INLINE {
+                if ((unsigned)(v - in0) < in_row)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc_smem(ring) + to), "l"(from) : "memory");
                 asm volatile("cp.async.commit_group;" ::: "memory");
+                from += 32 * VE;
             };
-            // positions in the ring go by base / 32, whatever v0 is
 #pragma unroll
-            for (int k = 0; k < SAMPLE_RING - 1; ++k) request(v0 + 32 * k);
-            for (int base = v0; base < v1; base += 32) {
-                request(base + 32 * (SAMPLE_RING - 1));
+            for (int k = 0; k < SAMPLE_RING - 1; ++k) request(v0 + lane + 32 * k, 512 * k);
+            for (int v = v0 + lane; v - lane < v1; v += 32) {
+                request(v + 32 * (SAMPLE_RING - 1), (slot + 512 * (SAMPLE_RING - 1)) % (512 * SAMPLE_RING));
                 asm volatile("cp.async.wait_group %0;" ::"n"(SAMPLE_RING - 1) : "memory");
-                const int v = base + lane;
-                if (v < v1 && inside(v)) {
-                    *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(ring + (base / 32 % SAMPLE_RING) * 512);
+                if ((unsigned)(v - in0) < in_row) {
+                    *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(ring + slot);
                 } else if (v < v1) {
                     load(v, e);
                 } else {
 #pragma unroll
                     for (int j = 0; j < VE; ++j) e[j] = T(-INFINITY);
                 }
+                slot = (slot + 512) % (512 * SAMPLE_RING);
                 if (odd) clean(e);
                 if (!f(v, e)) break;
             }
