@@ -25,8 +25,9 @@
 //   the row again, 623 so).
 //
 // What bounds it.  One row of 32000 (top-k 50 and top-p: 10 us): a dozen phases of 0.3 to 2 us each, cluster barriers and reads
-// of another CTA's memory.  512 rows of 128000 in FP32 (top-p 0.95: 375 us; their 262 MB take 40 us): instructions, some 140
-// for a logit, three quarters of the issue slots, the exponential in 64 bits a third of them (FP64 is a tenth busy, DRAM too).
+// of another CTA's memory.  512 rows of 128000 in FP32 (top-p 0.95: 290 us for N(0, 16), 573 for N(0, 4); their 262 MB take
+// 40 us): instructions, some 105 for a logit of the former, 71 % of the issue slots (FP64 is a seventh busy).  The largest
+// logit and the sum of all weights, without a rule, take 55 of them and 212 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     const auto refine = [&](int step, bool by_mass, unsigned count, double target, u64 before, bool sum_front) SAMPLE_INLINE {
         unsigned n = 0;
         front = 0.0;
-        fronted = sum_front;
+        fronted = !STAGED && sum_front;   // of a row in shared memory the saving is lost on registers (32000 logits: 10.2 us, 9.9)
         if (STAGED || here) {
             for (int i = lane; i < held; i += 32) {
                 const float v = to_float(mine[i]);

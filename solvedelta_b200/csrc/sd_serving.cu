@@ -213,8 +213,8 @@ int launch_sample(SampleParams p, long long rows, cudaStream_t stream) {
 template <class T>
 int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
     // as many CTAs a row as the SMs take at once, two on each, with 2048 entries at least; and so many that the rows in work
-    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32, top-p: 552 us with one CTA a row, 398 with
-    // two, 492 with four)
+    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32, top-p 0.95, logits N(0, 4): 645 us with one
+    // CTA a row, 573 with two, 660 with four; N(0, 16): 287, 291, 365)
     const auto worth = [&](int c) {
         return p.V >= c * 2048 && (rows * c <= 2 * 148 || 2 * 148 / (c / 2) * (long long)p.V * (int)sizeof(T) > SAMPLE_L2);
     };

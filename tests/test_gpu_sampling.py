@@ -63,6 +63,26 @@ def test_borders_among_thousands_of_candidates(dtype, rows, vocab):
             assert torch.equal(sd.sample_tokens(logits, u, **settings), first)
 
 
+@pytest.mark.parametrize("dtype,rows,vocab", ((torch.float32, 3, 262143), (torch.bfloat16, 160, 120007)))
+def test_more_stay_than_shared_memory_takes(dtype, rows, vocab):
+    """Flat rows that are read again: most of them stay; a border's step of some hundred entries, of thousands, of equal ones,
+    under masks."""
+    logits, u = _logits(rows, vocab, 31, dtype, 0.6)
+    few_values = (logits.float() * 4).round().to(dtype) / 4   # thousands of ties on the border
+    masked = logits.clone()
+    masked[:, 1000::5] = -math.inf
+    masked[:, ::1001] = math.nan
+    uneven = logits.clone()
+    uneven[:, : vocab // 2] += 3.0   # one half is in front of the border, the other spreads over it
+    for x in (logits, few_values, masked, uneven):
+        for settings in (dict(top_p=0.9), dict(top_p=0.6, temperature=0.3), dict(top_p=0.95, min_p=1e-3), dict(top_k=90001),
+                         dict(top_k=100000, top_p=0.97)):
+            first = sd.sample_tokens(x, u, **settings)
+            assert first[::53].tolist() == ref.tokens(x[::53], u[::53], **settings)
+            for _ in range(3):
+                assert torch.equal(sd.sample_tokens(x, u, **settings), first)
+
+
 def test_a_number_and_a_tensor_of_it_draw_the_same():
     logits, u = _logits(50, 9000, 4)
     for name, value in (("temperature", 0.7), ("top_p", 0.95), ("min_p", 0.01), ("top_k", 700)):
