@@ -15,7 +15,7 @@
 // in shared memory; of long ones (many rows of a large vocabulary) every pass reads the row again, out of L2, through a ring
 // of asynchronous copies.
 // A rule first takes a histogram of the row over steps of a 16th of a binade of the weight, of counts (top-k) or of weights to 16
-// bits (top-p), which says in which step its border lies at most.  What is in front of that is all that can be drawn:
+// bits (14 in long slices; top-p), which says in which step its border lies at most.  What is in front of that is all that can be drawn:
 // * up to 512 candidates go to the first CTA, one a thread, which sorts them, sums them up and draws;
 // * more are moved together by their warps.  The exact border comes from the entries of its step, gathered, or, where those
 //   are more than 512, from further histograms over equal steps of the logit's bits, until one value is left; sums and draw
@@ -64,7 +64,9 @@ constexpr int SAMPLE_BIN_BITS = 3;        // eight of them are a bin
 constexpr float SAMPLE_FAR = 63.9f;       // binades, where the last bin ends
 static_assert(int(SAMPLE_FAR * SAMPLE_TABLE) >> SAMPLE_BIN_BITS < SAMPLE_BINS, "bins");
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
+constexpr int SAMPLE_MAX_SLICE = 180000;  // elements: longer rows are shared by two CTAs at least
 constexpr int SAMPLE_RING = 4;            // vectors a lane has in flight, where the row is read again
+constexpr size_t SAMPLE_STAGED = 94 * 1024;     // bytes of a slice that is kept in shared memory: two CTAs share an SM
 constexpr size_t SAMPLE_RING_BYTES = size_t(SAMPLE_THREADS) * 16 * SAMPLE_RING;
 typedef unsigned long long u64;
 // the kernel's parts share its variables by reference: one that is not inlined would keep them in local memory
@@ -833,20 +835,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         else if (step >= 0) rule = TOP_K;
         if (by_p && rule == DONE) rule = TOP_P_LEFT;
     } else if (by_p) {
-        // the sum of all weights, and a histogram of their upper 16 bits (against 2^(43 - a), the binade of the bin): its
-        // running sums are not above the true ones, so the border is not behind the bin in which they reach the target
-        constexpr int PER_BINADE = SAMPLE_TABLE >> SAMPLE_BIN_BITS;
+        // the sum of all weights, and a histogram of their upper 16 bits (against 2^(43 - a), the binade of the bin), or of 14, so that
+        // a counter of 32 bits takes a slice of equal logits: its running sums are not above the true ones, so the border is not
+        // behind the bin in which they reach the target
+        constexpr int PER_BINADE = SAMPLE_TABLE >> SAMPLE_BIN_BITS, BITS = STAGED ? 16 : 14;
+        static_assert((u64)(STAGED ? SAMPLE_STAGED / sizeof(T) : SAMPLE_MAX_SLICE) * 129 / 128 << BITS < 1ull << 32,
+                      "an entry counts 2^BITS, or half a table step more at the end of a binade");
         double sum = 0.0;
         each_loaded([&](float v) {
             const int n = whole_steps(v);
             const double w = weight_at(v, n);
             sum += w;
             const int high = __double2hiint(w), binades = (high >> 20) - (1023 + 43) + (n >> 7);   // over 2^(43 - a): 0, or 1 at its end
-            if (high != 0) atomicAdd(&sh.count[n >> SAMPLE_BIN_BITS], (unsigned)((high & 0xfffff) | 0x100000) << (binades + 1) >> 6);
+            if (high != 0) atomicAdd(&sh.count[n >> SAMPLE_BIN_BITS], (unsigned)((high & 0xfffff) | 0x100000) << (binades + 1) >> (22 - BITS));
         });
         block_sum((u64)sum);
         for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
-            const int up = SAMPLE_WEIGHT_BITS - 1 - 15 - b / PER_BINADE;
+            const int up = SAMPLE_WEIGHT_BITS - BITS - b / PER_BINADE;
             sh.mass[b] = up >= 0 ? (u64)sh.count[b] << up : (u64)sh.count[b] >> -up;
         }
         publish(false, true);

@@ -193,7 +193,6 @@ bool token_fuses(const sd_int8_linear_args* a) {
 size_t q_bytes(const sd_int8_linear_args* a) { return ((size_t)a->rows * padded(a->K) + 255) / 256 * 256; }
 
 // ---- sampling ----
-constexpr size_t SAMPLE_STAGED = 94 * 1024;     // bytes of a slice that is kept in shared memory: two CTAs share an SM
 constexpr size_t SAMPLE_LIST_BYTES = 60 * 1024;
 constexpr long long SAMPLE_L2 = 96 << 20;       // of 126 MB
 static_assert(2 * (SAMPLE_STAGED + sizeof(SampleShared) + 1024) <= 228 * 1024 &&
@@ -218,6 +217,8 @@ int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
     const auto worth = [&](int c) {
         return p.V >= c * 2048 && (rows * c <= 2 * 148 || 2 * 148 / (c / 2) * (long long)p.V * (int)sizeof(T) > SAMPLE_L2);
     };
+    static_assert(SAMPLE_L2 / (2 * 148 * (int)sizeof(T)) + 16 <= SAMPLE_MAX_SLICE && SAMPLE_MAX_VOCAB / 2 + 16 <= SAMPLE_MAX_SLICE,
+                  "longest row of one CTA, longest part of two");
     if (worth(8)) return launch_sample<T, 8>(p, rows, stream);
     if (worth(4)) return launch_sample<T, 4>(p, rows, stream);
     if (worth(2)) return launch_sample<T, 2>(p, rows, stream);

@@ -266,3 +266,18 @@ def test_refusals():
         sd.sample_tokens(logits, u, top_p=torch.ones(4))
     with pytest.raises(TypeError, match="whole numbers"):
         sd.sample_tokens(logits, u, top_k=torch.ones(4, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", ((torch.float32, 160, 70000), (torch.bfloat16, 256, 128000), (torch.bfloat16, 300, 170001), (torch.float32, 3, 262144)))
+def test_flat_rows_of_more_entries_than_a_short_counter_takes(dtype, rows, vocab):
+    """Equal and nearly equal logits, tens of thousands of them in one step and one CTA, top-p with and without min-p."""
+    u = ((torch.arange(rows, device="cuda") % 16 + 0.4) / 16).float()
+    equal = torch.full((rows, vocab), -2.5, dtype=dtype, device="cuda")
+    two = equal.clone()
+    two[:, 7::3] = -1.0
+    for x in (equal, two):
+        for settings in (dict(top_p=0.5, min_p=0.1), dict(top_p=0.9, min_p=0.05), dict(top_p=0.5), dict(top_p=0.97, temperature=1e20, min_p=0.5),
+                         dict(top_p=0.4, top_k=vocab - 10, min_p=0.1), dict(top_p=0.5, min_p=0.3)):
+            got = sd.sample_tokens(x, u, **settings)
+            assert got[:16].tolist() == ref.tokens(x[:16], u[:16], **settings)
+            assert torch.equal(got[16:], got[:16].repeat(-(-rows // 16))[16:rows])
