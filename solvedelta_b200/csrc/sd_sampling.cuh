@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         find(0, group_masses, masses, [&](u64 a, u64 b) { return (double)a < target && !((double)b < target); });
         step = sh.bin < 0 ? SAMPLE_BINS - 1 : sh.bin;
         keep = min(step, min_p_bin);
-        if (step <= min_p_bin) rule = TOP_P;   // else min-p cuts in front of the border
+        if (step <= min_p_bin) rule = TOP_P;
     } else {
         keep = min_p_bin;
     }
@@ -869,6 +869,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     if (keep < SAMPLE_BINS && keep_up_to(keep)) {
         draw_from_list(by_k ? (unsigned)top_k : SAMPLE_THREADS, by_p, target, by_k);
         return;
+    }
+    if (by_p && !by_k && step > min_p_bin) {
+        // min-p cuts in front of the last step in which top-p's border can lie.  The border is behind all that is left if the first
+        // step in which it can lie is: of a weight the histogram lost less than its 2^-(BITS - 1) (2^-13 at most), of a bin
+        // of a slice less than one (8192 in all)
+        const double least = target * (1.0 - 0x1p-13) - 0x1p14;
+        find(0, group_masses, masses, [&](u64, u64 b) { return !((double)b < least); });
+        if (sh.bin >= 0 && sh.bin <= min_p_bin) rule = TOP_P_LEFT;
     }
     while (rule != DONE) {
         if (rule == TOP_P_LEFT) {
@@ -892,6 +900,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             publish(true, true);
             find(0, group_masses, masses, [&](u64 a, u64 b) { return (double)a < target && !((double)b < target); });
             step = sh.bin;
+            if (step < 0) break;   // min-p cut in front of the border
         }
         const bool found = refine(step, rule != TOP_K, (unsigned)top_k, target, rule == TOP_K ? in_front_of_step : rule == TOP_P ? 0 : sh.before,
                                   rule == TOP_P);

@@ -281,3 +281,20 @@ def test_flat_rows_of_more_entries_than_a_short_counter_takes(dtype, rows, vocab
             got = sd.sample_tokens(x, u, **settings)
             assert got[:16].tolist() == ref.tokens(x[:16], u[:16], **settings)
             assert torch.equal(got[16:], got[:16].repeat(-(-rows // 16))[16:rows])
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,spread", ((torch.float32, 24, 128000, 0.5), (torch.bfloat16, 24, 128000, 0.5), (torch.float32, 200, 40000, 0.4),
+                                                     (torch.bfloat16, 2, 32000, 0.3)))
+def test_top_p_next_to_one_beside_min_p(dtype, rows, vocab, spread):
+    """Flat rows whose top-p border lies at their end, close in front of what min-p takes or behind it."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    row = (spread * torch.randn(1, vocab, generator=gen, device="cuda")).to(dtype)
+    u = ((torch.arange(24, device="cuda") + 0.5) / 24).float().repeat(-(-rows // 24))[:rows].contiguous()
+    logits = row.expand(rows, vocab).contiguous()
+    weights = (row[0].double() - row.max().double()).exp().sort().values.cpu()
+    for smallest in (0, 5, 40):   # min-p at the smallest weight (nothing goes), and at others in front of it
+        min_p = float(weights[smallest]) * 0.999
+        for top_p in (0.999, 0.9999, 0.99999, 0.999995, 1 - 2 ** -24):
+            got = sd.sample_tokens(logits, u, top_p=top_p, min_p=min_p)
+            assert got[:24].tolist() == ref.tokens(logits[:24], u[:24], top_p=top_p, min_p=min_p)
+            assert torch.equal(got[24:], got[:24].repeat(-(-rows // 24))[24:rows])
