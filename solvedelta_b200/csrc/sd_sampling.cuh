@@ -15,7 +15,7 @@
 // in shared memory; of long ones (many rows of a large vocabulary) every pass reads the row again, out of L2, through a ring
 // of asynchronous copies.
 // A rule first takes a histogram of the row over steps of a 16th of a binade of the weight, of counts (top-k) or of weights to 16
-// bits (14 in long slices; top-p), which says in which step its border lies at most.  What is in front of that is all that can be drawn:
+// bits (15 or 14 in long slices; top-p), which says in which step its border lies at most.  What is in front of that is all that can be drawn:
 // * up to 512 candidates go to the first CTA, one a thread, which sorts them, sums them up and draws;
 // * more are moved together by their warps.  The exact border comes from the entries of its step, gathered, or, where those
 //   are more than 512, from further histograms over equal steps of the logit's bits, until one value is left; sums and draw
@@ -64,9 +64,20 @@ constexpr int SAMPLE_BIN_BITS = 3;        // eight of them are a bin
 constexpr float SAMPLE_FAR = 63.9f;       // binades, where the last bin ends
 static_assert(int(SAMPLE_FAR * SAMPLE_TABLE) >> SAMPLE_BIN_BITS < SAMPLE_BINS, "bins");
 constexpr int SAMPLE_MAX_VOCAB = 1 << 18;
-constexpr int SAMPLE_MAX_SLICE = 180000;  // elements: longer rows are shared by two CTAs at least
-constexpr int SAMPLE_RING = 4;            // vectors a lane has in flight, where the row is read again
 constexpr size_t SAMPLE_STAGED = 94 * 1024;     // bytes of a slice that is kept in shared memory: two CTAs share an SM
+// Elements of a slice that is read again: longer rows are shared by more CTAs.
+template <class T>
+constexpr int SAMPLE_MAX_SLICE = sizeof(T) == 4 ? 90000 : 180000;
+// Bits of a weight in the first histogram of top-p, as many as leave a counter of 32 bits room for a slice of equal logits: one
+// counts 2^bits, or half a table step more at the end of a binade.  (Few bits miss the border's step more often, and a row that
+// does ends with a histogram of whole weights: 512 rows of 128000, FP32, N(0, 4), top-p 0.95: 522 us with 16,
+// 537 with 15, 580 with 14.)
+template <class T, bool STAGED>
+constexpr int SAMPLE_BIN_WEIGHT_BITS = STAGED ? 16 : sizeof(T) == 4 ? 15 : 14;
+template <class T, bool STAGED>
+constexpr bool SAMPLE_COUNTERS_HOLD =
+    (unsigned long long)(STAGED ? SAMPLE_STAGED / sizeof(T) : SAMPLE_MAX_SLICE<T>) * 129 / 128 << SAMPLE_BIN_WEIGHT_BITS<T, STAGED> < 1ull << 32;
+constexpr int SAMPLE_RING = 4;            // vectors a lane has in flight, where the row is read again
 constexpr size_t SAMPLE_RING_BYTES = size_t(SAMPLE_THREADS) * 16 * SAMPLE_RING;
 typedef unsigned long long u64;
 // the kernel's parts share its variables by reference: one that is not inlined would keep them in local memory
@@ -835,12 +846,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
         else if (step >= 0) rule = TOP_K;
         if (by_p && rule == DONE) rule = TOP_P_LEFT;
     } else if (by_p) {
-        // the sum of all weights, and a histogram of their upper 16 bits (against 2^(43 - a), the binade of the bin), or of 14, so that
-        // a counter of 32 bits takes a slice of equal logits: its running sums are not above the true ones, so the border is not
-        // behind the bin in which they reach the target
-        constexpr int PER_BINADE = SAMPLE_TABLE >> SAMPLE_BIN_BITS, BITS = STAGED ? 16 : 14;
-        static_assert((u64)(STAGED ? SAMPLE_STAGED / sizeof(T) : SAMPLE_MAX_SLICE) * 129 / 128 << BITS < 1ull << 32,
-                      "an entry counts 2^BITS, or half a table step more at the end of a binade");
+        // the sum of all weights, and a histogram of their upper bits (against 2^(43 - a), the binade of the bin), as many as leave a
+        // counter of 32 bits room for a slice of equal logits: its running sums are not above the true ones, so the border is
+        // not behind the bin in which they reach the target
+        constexpr int PER_BINADE = SAMPLE_TABLE >> SAMPLE_BIN_BITS;
+        constexpr int BITS = SAMPLE_BIN_WEIGHT_BITS<T, STAGED>;
+        static_assert(SAMPLE_COUNTERS_HOLD<T, STAGED>, "histogram of weights");
         double sum = 0.0;
         each_loaded([&](float v) {
             const int n = whole_steps(v);
@@ -872,7 +883,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
     }
     if (by_p && !by_k && step > min_p_bin) {
         // min-p cuts in front of the last step in which top-p's border can lie.  The border is behind all that is left if the first
-        // step in which it can lie is: of a weight the histogram lost less than its 2^-(BITS - 1) (2^-13 at most), of a bin
+        // step in which it can lie is: of a weight the histogram lost less than its 2^-(BITS - 1), 2^-13 at most, of a bin
         // of a slice less than one (8192 in all)
         const double least = target * (1.0 - 0x1p-13) - 0x1p14;
         find(0, group_masses, masses, [&](u64, u64 b) { return !((double)b < least); });

@@ -217,8 +217,8 @@ int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
     const auto worth = [&](int c) {
         return p.V >= c * 2048 && (rows * c <= 2 * 148 || 2 * 148 / (c / 2) * (long long)p.V * (int)sizeof(T) > SAMPLE_L2);
     };
-    static_assert(SAMPLE_L2 / (2 * 148 * (int)sizeof(T)) + 16 <= SAMPLE_MAX_SLICE && SAMPLE_MAX_VOCAB / 2 + 16 <= SAMPLE_MAX_SLICE,
-                  "longest row of one CTA, longest part of two");
+    // by the second condition no part of a row is longer than this
+    static_assert(SAMPLE_L2 / (2 * 148 * (int)sizeof(T)) + 16 <= SAMPLE_MAX_SLICE<T>, "longest slices");
     if (worth(8)) return launch_sample<T, 8>(p, rows, stream);
     if (worth(4)) return launch_sample<T, 4>(p, rows, stream);
     if (worth(2)) return launch_sample<T, 2>(p, rows, stream);
