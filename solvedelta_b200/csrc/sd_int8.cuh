@@ -26,13 +26,13 @@ struct QuantizeParams {
 // What a row's largest magnitude (its bits) makes of the row.
 struct RowScale {
     float scale, inverse, largest;   // a / 127, about 127 / a, a
-    bool bad, special;               // not finite; that, or so small that the inverse may overflow
+    bool bad, special;               // not finite; that, or at either end of FP32's range: see quantize_extreme
 };
 __device__ __forceinline__ RowScale row_scale(unsigned largest_bits) {
     RowScale r;
     r.largest = __uint_as_float(largest_bits);
     r.bad = largest_bits >= 0x7f800000u;
-    r.special = r.bad || r.largest < 1e-30f;
+    r.special = r.largest < 1e-30f || !(r.largest < 2.5e36f);
     r.scale = r.bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(r.largest, 127.f);
     r.inverse = r.special ? 0.f : __fdiv_rn(127.f, r.largest);
     return r;
@@ -47,8 +47,8 @@ __device__ __forceinline__ int quantize_exactly(float x, float inverse, float a)
     const int n = (int)low;
     return n + (above || (tie && (n & 1)) ? 1 : 0);
 }
-// The same for rows whose inverse may overflow.
-__device__ __noinline__ int quantize_tiny(float x, float a) { return a == 0.f ? 0 : (int)rint(127.0 * (double)x / (double)a); }
+// The same for rows whose inverse, or whose 127 x, may overflow.  (A quotient that is not a half is 2^-40 of itself or more off one.)
+__device__ __noinline__ int quantize_extreme(float x, float a) { return a == 0.f ? 0 : (int)rint(127.0 * (double)x / (double)a); }
 
 template <class T>
 __device__ __forceinline__ float to_float(T v);
@@ -125,7 +125,7 @@ __device__ __forceinline__ uint2 quantize_piece(const Piece<T>& p, const RowScal
             for (int i = 0; i < 8; ++i) u[i] = (unsigned)(quantize_exactly(v[i], r.inverse, r.largest) + 128) << 16;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = (unsigned)((r.bad ? 0 : quantize_tiny(v[i], r.largest)) + 128) << 16;
+            for (int i = 0; i < 8; ++i) u[i] = (unsigned)((r.bad ? 0 : quantize_extreme(v[i], r.largest)) + 128) << 16;
         }
     }
     uint2 out;

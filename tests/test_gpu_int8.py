@@ -252,3 +252,27 @@ def test_refusals():
         sd.quantize_rows(torch.zeros(1, 131073, device="cuda"))
     with pytest.raises(ValueError, match="bias must be"):
         sd.int8_linear(x, weight, weight_scale, weight_scale[:5])
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("largest", (2.0e36, 2.6e36, 2.69e36, 1e38, 3.0e38, 3.38e38))
+def test_rows_of_very_large_finite_entries(largest, dtype):
+    """Up to the end of FP32's range, halves and entries off a half in one group of eight."""
+    gen = torch.Generator(device="cuda").manual_seed(int(largest / 1e35))
+    shares = torch.tensor([1, .5, .9, .8953, -.3, .56, .77, .11], device="cuda")
+    steps = torch.arange(1, 17, device="cuda") / 16
+    x = torch.cat((shares, steps, -steps, 2 * torch.rand(512 - 40, generator=gen, device="cuda") - 1)) * largest
+    x = torch.stack((x, x.roll(3), -x, x.flip(0))).to(dtype)
+    assert torch.isfinite(x).all()
+    want, want_scale = ref.quantize(ref.as64(x))
+    q, scale = sd.quantize_rows(x)
+    assert np.array_equal(q.cpu().numpy(), want) and np.array_equal(ref.as64(scale), want_scale)
+    odd = sd.quantize_rows(x[:, 1:])[0]   # rows that start anywhere
+    assert np.array_equal(odd.cpu().numpy(), ref.quantize(ref.as64(x[:, 1:]))[0])
+    # one row quantised inside the product, four in front of it, many in tiles: the unit matrix shows the integers
+    unit = torch.eye(512, dtype=torch.int8, device="cuda")
+    ones = torch.ones(512, device="cuda")
+    for rows in (x[:1], x, x.repeat(10, 1)):
+        y = ref.as64(sd.int8_linear(rows, unit, ones, out_dtype=torch.float32))
+        whole, unit_of = ref.quantize(ref.as64(rows))
+        assert (np.abs(y - whole * unit_of[:, None]) <= 2.0 ** -24 * np.abs(whole) * unit_of[:, None]).all()
