@@ -28,6 +28,9 @@ Tensor readable(const Tensor& rows) {
 }
 
 void require_no_gradient(std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)   // tangents pass whether gradients are recorded or not
+        if (t->defined() && t->_fw_grad(0).defined())
+            throw std::runtime_error("8-bit projections have no forward-mode derivative: call them on tensors without tangents");
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor* t : tensors)
         if (t->defined() && t->requires_grad())

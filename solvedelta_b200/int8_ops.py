@@ -1,5 +1,6 @@
 """Projections with 8-bit weights and activations for serving: rows of int8 with a scale for each token and each
-output channel, the products exact in 32-bit integers (csrc/sd_int8.cuh).  No reverse pass, no fallback.
+output channel, the products exact in 32-bit integers (csrc/sd_int8.cuh).  No reverse pass, no forward-mode
+derivative (both are refused), no fallback.
 
 A row stands for ``q * scale`` with ``scale = max|x| / 127`` and ``q = 127 x / max|x|`` rounded to the nearest whole
 number (ties to even); weights are quantised the same way, a scale for each output channel.
@@ -17,7 +18,8 @@ from . import _lib
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of the rows of ``x`` ``[..., K]`` (BF16 or FP32 CUDA): ``q`` int8 ``[..., K]``, its rows padded to
     whole groups of 16 bytes, ``scale`` FP32 ``[...]``.  A row of zeros has scale 0; a row with an infinity or a NaN has
-    ``q = 0`` and scale NaN, so that everything computed from it is NaN.  Neither output carries a gradient."""
+    ``q = 0`` and scale NaN, so that everything computed from it is NaN.  Neither output carries a gradient or a
+    tangent."""
     return _lib.host().quantize_rows(x)
 
 

@@ -276,3 +276,21 @@ def test_rows_of_very_large_finite_entries(largest, dtype):
         y = ref.as64(sd.int8_linear(rows, unit, ones, out_dtype=torch.float32))
         whole, unit_of = ref.quantize(ref.as64(rows))
         assert (np.abs(y - whole * unit_of[:, None]) <= 2.0 ** -24 * np.abs(whole) * unit_of[:, None]).all()
+
+
+def test_forward_mode_tangents_are_refused():
+    weight, weight_scale = _weight(32, 64, 1)
+    x = _rows(4, 64, 1)
+    q, scale = sd.quantize_rows(x)
+    bias = torch.zeros(32, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = {name: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+                for name, t in (("x", x), ("scale", scale), ("weight_scale", weight_scale), ("bias", bias))}
+        for call in (lambda: sd.int8_linear(dual["x"], weight, weight_scale), lambda: sd.int8_linear(x, weight, dual["weight_scale"]),
+                     lambda: sd.int8_linear(x, weight, weight_scale, dual["bias"]), lambda: sd.int8_matmul(q, dual["scale"], weight, weight_scale),
+                     lambda: sd.int8_gated_mlp(dual["x"], weight, weight_scale, None, weight[:, :16], weight_scale, None)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            sd.int8_linear(dual["x"], weight, weight_scale)
+        sd.int8_linear(x, weight, weight_scale)
