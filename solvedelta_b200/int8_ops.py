@@ -51,9 +51,11 @@ def int8_gated_mlp(x: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor, up
 class Int8Linear(nn.Module):
     """A projection for inference whose weight is held in int8 with a scale for each output channel (buffers ``weight``
     ``[out, in]``, ``weight_scale`` ``[out]`` and, where there is one, ``bias``); the rows it is given are quantised row by
-    row on the way in.  Not trainable: with gradients recorded for its input it raises."""
+    row on the way in, the result is BF16.  ``bias`` is BF16 or FP32 (``bias_dtype``).  Not trainable: with gradients
+    recorded for its input it raises."""
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = False, device=None) -> None:
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, device=None,
+                 bias_dtype: torch.dtype = torch.bfloat16) -> None:
         super().__init__()
         self.in_features, self.out_features = in_features, out_features
         # rows start on 16-byte boundaries, as the kernels read them
@@ -61,13 +63,15 @@ class Int8Linear(nn.Module):
         weight = torch.zeros(out_features, pitch, dtype=torch.int8, device=device)[:, :in_features]
         self.register_buffer("weight", weight)
         self.register_buffer("weight_scale", torch.zeros(out_features, dtype=torch.float32, device=device))
-        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.bfloat16, device=device) if bias else None)
+        self.register_buffer("bias", torch.zeros(out_features, dtype=bias_dtype, device=device) if bias else None)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
-        """The projection of a CUDA ``nn.Linear`` (BF16 or FP32), its weight quantised output channel by output channel."""
+        """The projection of a CUDA ``nn.Linear`` (BF16 or FP32), its weight quantised output channel by output channel, its
+        bias as it is."""
         weight = linear.weight.detach()
-        made = cls(linear.in_features, linear.out_features, linear.bias is not None, weight.device)
+        made = cls(linear.in_features, linear.out_features, linear.bias is not None, weight.device,
+                   torch.bfloat16 if linear.bias is None or linear.bias.dtype == torch.bfloat16 else torch.float32)
         q, scale = quantize_rows(weight)
         if not torch.isfinite(scale).all():
             raise ValueError("a weight with infinities or NaNs cannot be quantised")

@@ -167,3 +167,20 @@ def test_draws_follow_the_generator():
     with pytest.raises(ValueError, match="max_new_tokens, B"):
         model.sample_generate(ids, 8, uniform=torch.rand(8, 3, device="cuda"))
     assert torch.equal(model.sample_generate(ids, 0), ids)
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_a_module_keeps_the_type_of_its_bias(dtype):
+    torch.manual_seed(4)
+    linear = nn.Linear(96, 40, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        linear.bias.copy_(torch.randn(40) + 1 / 3)
+    made = sd.Int8Linear.from_linear(linear)
+    assert made.bias.dtype == dtype and torch.equal(made.bias, linear.bias.detach())
+    x = torch.randn(5, 96, device="cuda").to(torch.bfloat16)
+    q, scale = sd.quantize_rows(linear.weight.detach())
+    assert torch.equal(made(x), sd.int8_linear(x, q, scale, linear.bias.detach()))
+    twin = sd.Int8Linear(96, 40, bias=True, device="cuda", bias_dtype=dtype)
+    twin.load_state_dict(made.state_dict())
+    assert torch.equal(twin(x), made(x))
+    assert copy.deepcopy(made).bfloat16().bias.dtype == torch.bfloat16 and copy.deepcopy(made).half().bias.dtype == torch.bfloat16
