@@ -495,7 +495,9 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
                              output_hidden_states=output_hidden_states, **kwargs)
         hidden_states = outputs.last_hidden_state
         keep_all = labels is not None or logits_to_keep in (None, 0)
-        fused_head = labels is not None and self.config.fuse_linear_cross_entropy
+        # (a head in int8 has no chunked form: its logits are made whole)
+        fused_head = (labels is not None and self.config.fuse_linear_cross_entropy
+                      and not isinstance(self.lm_head, Int8Linear))
         logits = None
         if not fused_head:
             logits = self.lm_head(hidden_states if keep_all else hidden_states[:, -logits_to_keep:])
@@ -512,7 +514,8 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
                 loss = fixed_dense_linear_cross_entropy(hidden_states, shifted, self.lm_head.weight,
                                                         self.lm_head.bias, ignore_index=self.ignore_index,
                                                         total=count)
-            elif self.config.fuse_cross_entropy and logits.is_cuda and logits.dtype == torch.bfloat16:
+            elif ((self.config.fuse_cross_entropy or self.config.fuse_linear_cross_entropy) and logits.is_cuda
+                  and logits.dtype == torch.bfloat16):
                 from .training import fused_cross_entropy   # two kernels on the BF16 logits, no FP32 copy
 
                 loss = fused_cross_entropy(logits, shifted, ignore_index=self.ignore_index)

@@ -144,6 +144,8 @@ def fixed_dense_linear_cross_entropy(x: torch.Tensor, target: torch.Tensor, weig
         raise ValueError("target must have the leading shape of x")
     if weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
         raise ValueError("weight must have shape [vocab, hidden]")
+    if not weight.is_floating_point():
+        raise TypeError("weight must be of a floating type: a head held in int8 has no chunked loss")
     return _FixedDenseLinearCrossEntropy.apply(x, target, weight, bias, ignore_index, total, num_chunks)
 
 

@@ -184,3 +184,24 @@ def test_a_module_keeps_the_type_of_its_bias(dtype):
     twin.load_state_dict(made.state_dict())
     assert torch.equal(twin(x), made(x))
     assert copy.deepcopy(made).bfloat16().bias.dtype == torch.bfloat16 and copy.deepcopy(made).half().bias.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("fused", (dict(fuse_linear_cross_entropy=True, fuse_cross_entropy=False), dict(fuse_cross_entropy=True),
+                                   dict(fuse_cross_entropy=False)))
+def test_loss_of_a_quantised_head(fused):
+    """The loss is that of the logits which the head gives, whichever way the configuration computes losses."""
+    model = _model(layers=1, **fused).quantize_int8(head=True)
+    ids = _ids(model, 2, 21)
+    labels = ids.clone()
+    labels[0, 4:9] = -100
+    with torch.no_grad():
+        loss = model(input_ids=ids, labels=labels).loss
+        logits = model(input_ids=ids).logits.double()
+    want = nn.functional.cross_entropy(logits[:, :-1].reshape(-1, 1000), labels[:, 1:].reshape(-1))
+    # FP32: a sum of 1000 exponentials is 1000 * 2^-24 of itself off at most, so its logarithm is 6e-5 off; the loss is near log 1000
+    assert abs(loss.item() - want.item()) <= 1e-4 * want.item()
+    if fused.get("fuse_linear_cross_entropy"):   # nothing counted: 0, as with a head in BF16
+        with torch.no_grad():
+            assert model(input_ids=ids, labels=torch.full_like(ids, -100)).loss.item() == 0.0
+    with torch.no_grad(), pytest.raises(TypeError, match="weight must be"):
+        sd.causal_lm_loss(model, ids, labels, total=35)
