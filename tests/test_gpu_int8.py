@@ -294,3 +294,15 @@ def test_forward_mode_tangents_are_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             sd.int8_linear(dual["x"], weight, weight_scale)
         sd.int8_linear(x, weight, weight_scale)
+
+
+@pytest.mark.parametrize("rows,width,columns", ((1, 1024, 520), (3, 33, 40), (16, 300, 128), (40, 1000, 96), (130, 77, 301)))
+def test_projection_of_fp32_rows(rows, width, columns):
+    x = _rows(rows, width, rows, torch.float32)
+    weight, weight_scale = _weight(columns, width, columns)
+    for given in (x, torch.cat((x, x), dim=1)[:, 1:width + 1], x.t().contiguous().t()):
+        q, scale = ref.quantize(ref.as64(given))
+        for out in (torch.bfloat16, torch.float32):
+            _check(sd.int8_linear(given, weight, weight_scale, out_dtype=out), q, scale, weight, weight_scale)
+            if columns % 2 == 0:
+                _check(sd.int8_linear(given, weight, weight_scale, swiglu=True, out_dtype=out), q, scale, weight, weight_scale, swiglu=True)
