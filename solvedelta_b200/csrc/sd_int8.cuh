@@ -660,9 +660,8 @@ __host__ __device__ constexpr long long int8_pitch(int K) { return ((long long)K
 
 struct Int8TokenParams {
     Int8Params o;              // M, outs, K, scales, bias, y
-    const void* x;             // rows, x_stride elements apart
+    const void* x;             // rows, x_stride elements apart, on 16-byte boundaries; K a multiple of eight in BF16
     long long x_stride;
-    int vec;                   // rows of x start on 16-byte boundaries
     const signed char* W;      // [N][w_stride], readable up to K rounded up to 16
     long long w_stride;
 };
@@ -680,8 +679,8 @@ __device__ __forceinline__ uint4 load_weight(const signed char* p) {
     return r;
 }
 
-// The rows of x as int8 in shared memory, zeros past K; T: BF16 or FP32 rows are quantised, int8 rows are copied.
-template <class T, bool VEC>
+// The rows of x as int8 in shared memory, zeros past K; T: BF16 rows are quantised, int8 rows are copied.
+template <class T>
 __device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char* s_q, float* s_scale, unsigned* s_top) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, M = p.o.M, K = p.o.K;
     const int pitch = (int)int8_pitch(K);
@@ -700,7 +699,7 @@ __device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char*
         const int segs = (pitch + 255) / 256, units = M * segs;
         const auto unit = [&](int u) {
             const int m = u / segs;
-            return load_piece<T, VEC>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, u < units ? (u - m * segs) * 256 + lane * 8 : K, K);
+            return load_piece<T, true>(reinterpret_cast<const T*>(p.x) + m * p.x_stride, u < units ? (u - m * segs) * 256 + lane * 8 : K, K);
         };
         const auto widen = [&](int u, const Piece<T>& piece) {
             if (u >= units) return;
@@ -730,7 +729,7 @@ __device__ __forceinline__ void int8_rows(const Int8TokenParams& p, signed char*
 }
 
 // RG: groups of eight rows; CG: groups of eight weight rows per CTA (2 with GATED)
-template <int RG, int CG, bool GATED, class T, bool VEC>
+template <int RG, int CG, bool GATED, class T>
 __global__ void __launch_bounds__(256, 2) k_int8_token(Int8TokenParams p) {
     static_assert(!GATED || CG == 2, "gate and value rows are the two groups");
     constexpr int KS = 8 / CG, MT = (RG + 1) / 2, B = I8_TOKEN_BATCH;
@@ -774,7 +773,7 @@ __global__ void __launch_bounds__(256, 2) k_int8_token(Int8TokenParams p) {
     for (int i = 0; i < I8_TOKEN_AHEAD; ++i) request(w[i]);
     chain_wait();
     chain_release();
-    int8_rows<T, VEC>(p, s_q, s_scale, s_top);
+    int8_rows<T>(p, s_q, s_scale, s_top);
     __syncthreads();
 
     // the columns that a thread finishes are the same ones of every tile

@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
             return false;
         }
         if (all <= SAMPLE_THREADS) {
-            // every CTA gets all entries of the step and sorts them
+            // every CTA gets all entries of the step and sorts them (they are in the lists: a warp's takes more than 512)
             unsigned at = before_slice + before_warp;
             const int on_hand = here ? held : stepped;
             for (int i0 = 0; i0 < on_hand; i0 += 32) {
@@ -713,19 +713,6 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) k_sample(SampleParams p) {
                     for (int r = 0; r < C; ++r) write(&sh.count[at + __popc(lanes & ((1u << lane) - 1))], r, order_bits(v));
                 at += __popc(lanes);
             }
-            if (on_hand < 0)
-                scan_range([&](int, const T (&e)[VE]) {
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) {
-                        const float v = to_float(e[j]);
-                        const bool in = v > -INFINITY && !(v < edge) && bin_of(v) == step;
-                        const unsigned lanes = __ballot_sync(0xffffffffu, in);
-                        if (in)
-                            for (int r = 0; r < C; ++r) write(&sh.count[at + __popc(lanes & ((1u << lane) - 1))], r, order_bits(v));
-                        at += __popc(lanes);
-                    }
-                    return true;
-                });
             everywhere();
             const unsigned key = sort_down(tid < all ? sh.count[tid] : 0u, all, sh.count);
             bool is_it = by_mass ? false : tid == count - 1 - (unsigned)before;

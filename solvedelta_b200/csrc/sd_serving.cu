@@ -160,27 +160,27 @@ int matmul(const Int8Params& p, const sd_int8_linear_args* a, const void* q, lon
 }
 
 size_t token_smem(int M, int K) { return (size_t)(M * int8_pitch(K)); }
-template <int RG, int CG, bool GATED, class T, bool VEC>
+template <int RG, int CG, bool GATED, class T>
 int launch_token(const Int8TokenParams& p, bool chained, cudaStream_t stream) {
     constexpr int WIDTH = GATED ? 8 : 8 * CG;
     const int tiles = (p.o.outs + WIDTH - 1) / WIDTH;
     const size_t smem = token_smem(p.o.M, p.o.K);
     const int resident = 148 * (smem <= 96 * 1024 ? 2 : 1);
-    return launch<k_int8_token<RG, CG, GATED, T, VEC>>((unsigned)(tiles < resident ? tiles : resident), 256, smem, I8_TOKEN_SMEM, 1,
+    return launch<k_int8_token<RG, CG, GATED, T>>((unsigned)(tiles < resident ? tiles : resident), 256, smem, I8_TOKEN_SMEM, 1,
                                                        chained, stream, p);
 }
-template <int RG, class T, bool VEC>
+template <int RG, class T>
 int token_width(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t stream) {
-    if (gated) return launch_token<RG, 2, true, T, VEC>(p, chained, stream);
+    if (gated) return launch_token<RG, 2, true, T>(p, chained, stream);
     // 16 columns a tile while that keeps most SMs busy (one row, 1024 x 2048: 2.9 us, with 8 columns 3.1; 2048 x 4096: 4.3 and 4.8),
     // else 8 (2816 x 1024: 3.2 us, with 16 columns 3.7)
-    return p.o.outs >= 16 * 128 ? launch_token<RG, 2, false, T, VEC>(p, chained, stream)
-                                : launch_token<RG, 1, false, T, VEC>(p, chained, stream);
+    return p.o.outs >= 16 * 128 ? launch_token<RG, 2, false, T>(p, chained, stream)
+                                : launch_token<RG, 1, false, T>(p, chained, stream);
 }
-template <class T, bool VEC>
+template <class T>
 int token_rows(const Int8TokenParams& p, bool gated, bool chained, cudaStream_t stream) {
-    if (p.o.M <= 8) return token_width<1, T, VEC>(p, gated, chained, stream);
-    return token_width<2, T, VEC>(p, gated, chained, stream);
+    if (p.o.M <= 8) return token_width<1, T>(p, gated, chained, stream);
+    return token_width<2, T>(p, gated, chained, stream);
 }
 bool token_takes(const sd_int8_linear_args* a) { return a->rows <= I8_TOKEN_ROWS && token_smem((int)a->rows, a->K) <= I8_TOKEN_SMEM; }
 // Few entries: every CTA quantises the rows for itself, which saves a launch; past that it costs more (4 x 1024 entries: 5.9 us
@@ -205,7 +205,9 @@ int launch_sample(SampleParams p, long long rows, cudaStream_t stream) {
     const size_t bytes = (size_t)p.slice * sizeof(T);
     if (bytes <= SAMPLE_STAGED)
         return launch<k_sample<T, C, true>>((unsigned)(rows * C), SAMPLE_THREADS, bytes, SAMPLE_STAGED, C, false, stream, p);
-    p.list = SAMPLE_LIST_BYTES / SAMPLE_WARPS / (sizeof(T) + sizeof(unsigned short));
+    constexpr int list = SAMPLE_LIST_BYTES / SAMPLE_WARPS / (sizeof(T) + sizeof(unsigned short));
+    static_assert(list > SAMPLE_THREADS, "what the CTAs sort fits into one warp's list");
+    p.list = list;
     constexpr size_t smem = SAMPLE_RING_BYTES + SAMPLE_LIST_BYTES;
     return launch<k_sample<T, C, false>>((unsigned)(rows * C), SAMPLE_THREADS, smem, smem, C, false, stream, p);
 }
@@ -263,7 +265,7 @@ int sd_int8_linear(const sd_int8_linear_args* a, void* stream_) {
     t.W = reinterpret_cast<const signed char*>(a->weight); t.w_stride = a->weight_stride;
     if (token_fuses(a)) {
         t.o = p; t.x = a->x; t.x_stride = a->x_stride;
-        return token_rows<__nv_bfloat16, true>(t, a->swiglu != 0, chained, stream);
+        return token_rows<__nv_bfloat16>(t, a->swiglu != 0, chained, stream);
     }
     const void* q = a->x;
     long long q_stride = a->x_stride;
@@ -281,7 +283,7 @@ int sd_int8_linear(const sd_int8_linear_args* a, void* stream_) {
     }
     if (token) {
         t.o = p; t.x = q; t.x_stride = q_stride;
-        return token_rows<signed char, true>(t, a->swiglu != 0, chained, stream);
+        return token_rows<signed char>(t, a->swiglu != 0, chained, stream);
     }
     return matmul(p, a, q, q_stride, chained, stream);
 }
