@@ -516,7 +516,8 @@ int sd_norm_gate_backward(const sd_norm_gate_args *args, void *stream);
  *                   scale = a / 127 and q_k = 127 x_k / a to the nearest whole number, ties to even.
  *                   A row of zeros has scale 0; one with an infinity or a NaN has q = 0 and scale NaN.
  * sd_int8_linear    y[i][j] = x_scale[i] weight_scale[j] sum_k q[i][k] weight[j][k] + bias[j], the sum exact
- *                   in int32, the rest in FP32, rounded once to the type of y.  x is either int8 (q, with
+ *                   in int32, the rest in FP32 (the sum times x_scale, times weight_scale, plus bias: infinite
+ *                   where one of these leaves FP32), rounded once to the type of y.  x is either int8 (q, with
  *                   x_scale) or BF16 / FP32, which is quantised first as sd_quantize_rows does.  With swiglu
  *                   y has N / 2 columns, silu(column j) * (column j + N / 2).
  *

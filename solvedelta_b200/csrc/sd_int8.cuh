@@ -95,8 +95,8 @@ template <class T>
 __device__ __forceinline__ unsigned whole_top(unsigned top) { return sizeof(T) == 2 ? max(top & 0xffff0000u, top << 16) : top; }
 
 // The entries as bytes.  With b = 384.5 + 2^-15 the sum 127 x / a + b has eight bits of q + 128 and 15 bits behind the point; the
-// product with the rounded inverse and the sum are off by less than 2^-15 together (1.5 * 2^-23 of 127, and half a unit), so q is
-// right unless those 15 bits are 0, 1 or 2, next to where it changes.
+// product with the inverse, which is rounded to 2^-24 of itself, and the sum are off by less than 2^-15 together (2^-17, and half a
+// unit: 2^-16), so q is right unless those 15 bits are 0, 1 or 2, next to where it changes.
 template <class T>
 __device__ __forceinline__ uint2 quantize_piece(const Piece<T>& p, const RowScale& r) {
     float v[8];

@@ -22,12 +22,13 @@
 //   go over what was moved;
 // * where that is too much for shared memory, the entries of the border's step alone are moved, and the weights in front of it
 //   are summed up once (512 rows of 128000, FP32, N(0, 4), top-p 0.95, 30000 kept of each: 1026 us when every histogram read
-//   the row again, 623 so).
+//   the row again, 623 with the first form of this).
 //
 // What bounds it.  One row of 32000 (top-k 50 and top-p: 10 us): a dozen phases of 0.3 to 2 us each, cluster barriers and reads
-// of another CTA's memory.  512 rows of 128000 in FP32 (top-p 0.95: 290 us for N(0, 16), 573 for N(0, 4); their 262 MB take
-// 40 us): instructions, some 105 for a logit of the former, 71 % of the issue slots (FP64 is a seventh busy).  The largest
-// logit and the sum of all weights, without a rule, take 55 of them and 212 us.
+// of another CTA's memory.  512 rows of 128000 in FP32 (top-p 0.95: 280 us for N(0, 16), 563 for N(0, 4); their 262 MB take
+// 40 us): instructions, some 105 for a logit of the former, 70 % of the issue slots (FP64 is a seventh busy).  The largest
+// logit and the sum of all weights, without a rule, take 55 of them and 207 us.  At 64 registers a thread some variables live
+// in local memory; one instruction of a thousand moves them.
 #pragma once
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -70,7 +71,7 @@ template <class T>
 constexpr int SAMPLE_MAX_SLICE = sizeof(T) == 4 ? 90000 : 180000;
 // Bits of a weight in the first histogram of top-p, as many as leave a counter of 32 bits room for a slice of equal logits: one
 // counts 2^bits, or half a table step more at the end of a binade.  (Few bits miss the border's step more often, and a row that
-// does ends with a histogram of whole weights: 512 rows of 128000, FP32, N(0, 4), top-p 0.95: 522 us with 16,
+// does ends with a histogram of whole weights: a batch of 512 rows of 128000, FP32, N(0, 4), top-p 0.95: 522 us with 16,
 // 537 with 15, 580 with 14.)
 template <class T, bool STAGED>
 constexpr int SAMPLE_BIN_WEIGHT_BITS = STAGED ? 16 : sizeof(T) == 4 ? 15 : 14;
@@ -129,7 +130,8 @@ __device__ __forceinline__ double fixed_power(int n, double r, const double* tab
     return n < SAMPLE_RANGE * SAMPLE_TABLE ? w : 0.0;   // farther entries have no r: they may be infinite
 }
 static_assert(SAMPLE_TABLE == 128, "fixed_power shifts by seven bits");
-static_assert(SAMPLE_MAX_VOCAB / SAMPLE_THREADS <= 512, "a lane's sum of weights is exact");
+static_assert(SAMPLE_MAX_SLICE<float> / SAMPLE_THREADS + 8 <= 512 && SAMPLE_MAX_SLICE<__nv_bfloat16> / SAMPLE_THREADS + 16 <= 512,
+              "a lane's sum of weights, of its share of the vectors and two more, is exact");
 
 // Shared memory of CTA `r` of the cluster, at the place of `p` in this one.
 __device__ __forceinline__ unsigned cluster_address(const void* p, int r) {

@@ -145,7 +145,8 @@ int matmul_tile(const Int8Params& p, const sd_int8_linear_args* a, const void* q
     };
     // Pairs of CTAs from half of the SMs on (700 x 2048 x 4096, 48 tiles: 11.3 us, tiles of one CTA 14.9; 300 x 2048 x 2048, 16
     // tiles: 10.9 against 8.5); else the wider tile while it gives every SM one (2048 x 1024 x 2816: 128 columns 13.5 us, 64 18.2;
-    // 128 x 1024 x 5632, 44 tiles of 128 columns: 6.4 against 5.9).
+    // 128 x 1024 x 5632, 44 tiles of 128 columns: 6.4 against 5.9).  Just under that bound the narrow tiles take a second round
+    // that is nearly empty (64 x 2048 x 11264 with SwiGLU, 88 tiles of 128 columns or 176 of 64: 13.5 us, 3.6 for its bytes).
     if (tiles(256, 256) >= 37 && p.M > 128) return launch_matmul<256, GATED, F32, true>(p, a, q, q_stride, chained, stream);
     if (tiles(128, 128) >= 148) return launch_matmul<128, GATED, F32, false>(p, a, q, q_stride, chained, stream);
     const int ctas_log2 = split_log2(tiles(128, 64), p.K);
@@ -214,8 +215,8 @@ int launch_sample(SampleParams p, long long rows, cudaStream_t stream) {
 template <class T>
 int sample(const SampleParams& p, long long rows, cudaStream_t stream) {
     // as many CTAs a row as the SMs take at once, two on each, with 2048 entries at least; and so many that the rows in work
-    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32, top-p 0.95, logits N(0, 4): 645 us with one
-    // CTA a row, 573 with two, 660 with four; N(0, 16): 287, 291, 365)
+    // at a time, which are read three times, stay in L2 (512 rows of 128000 in FP32, top-p 0.95, logits N(0, 4): 618 us with one
+    // CTA a row, 563 with two, 648 with four; N(0, 16): 277, 280, 354)
     const auto worth = [&](int c) {
         return p.V >= c * 2048 && (rows * c <= 2 * 148 || 2 * 148 / (c / 2) * (long long)p.V * (int)sizeof(T) > SAMPLE_L2);
     };

@@ -28,7 +28,8 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``y[..., j] = scale[...] * weight_scale[j] * sum_k q[..., k] weight[j, k] + bias[j]``: ``q`` int8 ``[..., K]``
     with FP32 ``scale`` ``[...]``, ``weight`` int8 ``[N, K]`` with FP32 ``weight_scale`` ``[N]``, ``bias`` BF16 or FP32
-    ``[N]``.  Sums are exact (``K`` up to 131072), the rest is FP32, rounded once to ``out_dtype`` (BF16 or FP32).  With
+    ``[N]``.  Sums are exact (``K`` up to 131072), the rest is FP32 (the sum times ``scale``, times ``weight_scale``,
+    plus ``bias``: infinite where one of these leaves FP32), rounded once to ``out_dtype`` (BF16 or FP32).  With
     ``swiglu`` the result is ``silu(y[..., :N/2]) * y[..., N/2:]``.  Rows as :func:`quantize_rows` makes them are read in
     place; others (an odd stride, an odd start) are copied first."""
     return _lib.host().int8_matmul(q, scale, weight, weight_scale, bias, swiglu, out_dtype)

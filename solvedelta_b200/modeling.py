@@ -436,9 +436,11 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
 
     def quantize_int8(self, head: bool = False) -> "SolveDeltaForCausalLM":
         """Hold the gated MLPs' weights, and with ``head`` the vocabulary projection's, in int8 (:class:`Int8Linear`), for
-        inference on a CUDA device: half of their bytes in a cached token, twice the tensor rate in a prompt.  The mixers
-        stay in BF16.  In place, not reversible; quantised modules are left as they are.  Checkpoints are those of the model
-        before: quantise after loading.  Returns the model."""
+        inference on a CUDA device: half of their bytes in a cached token, twice the tensor rate in a prompt.  A short
+        cached token is bound by launches, of which an int8 layer has more: one sequence at hidden size 1024 takes longer
+        than in BF16 (194 against 175 us, six layers), at 2048 less (361 against 382).  The mixers stay in BF16.  In place,
+        not reversible; quantised modules are left as they are.  Checkpoints are those of the model before: quantise after
+        loading.  A head in int8 has no chunked loss: its logits are made whole.  Returns the model."""
         if head and self.config.tie_word_embeddings:
             raise ValueError("a tied head shares the embedding's weight and cannot be quantised")
         for layer in self.model.layers:
