@@ -69,7 +69,11 @@ class Int8Linear(nn.Module):
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
         """The projection of a CUDA ``nn.Linear`` (BF16 or FP32), its weight quantised output channel by output channel, its
-        bias as it is."""
+        bias as it is.  A module that does more than its product (a subclass, an adapter, a parametrisation, a hook) is
+        refused: that part would be lost."""
+        if (type(linear) is not nn.Linear or "forward" in linear.__dict__ or linear._forward_hooks
+                or linear._forward_pre_hooks):
+            raise TypeError("only a plain nn.Linear without hooks can be held in int8")
         weight = linear.weight.detach()
         made = cls(linear.in_features, linear.out_features, linear.bias is not None, weight.device,
                    torch.bfloat16 if linear.bias is None or linear.bias.dtype == torch.bfloat16 else torch.float32)

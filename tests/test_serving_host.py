@@ -76,3 +76,26 @@ def test_argument_errors_are_status_codes(lib):
 
     assert [sample(logits=None), sample(V=0), sample(uniform=None), sample(logits_type=_lib.I8), sample(logits=at + 2)] == [-1] * 5
     assert sample(V=262145) == -2
+
+
+def test_projections_that_do_more_than_their_product_are_refused():
+    class Scaled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    hooked = torch.nn.Linear(16, 16)
+    handle = hooked.register_forward_hook(lambda module, args, out: 2 * out)
+    parametrised = torch.nn.utils.parametrizations.weight_norm(torch.nn.Linear(16, 16))
+    replaced = torch.nn.Linear(16, 16)
+    replaced.forward = lambda x: x
+    for module in (Scaled(16, 16), hooked, parametrised, replaced):
+        with pytest.raises(TypeError, match="plain nn.Linear"):
+            sd.Int8Linear.from_linear(module)
+    handle.remove()
+    with pytest.raises(TypeError, match="CUDA"):   # plain again: what is refused now is the device
+        sd.Int8Linear.from_linear(hooked)
+
+
+def test_chunked_loss_refuses_whole_numbers():
+    with pytest.raises(TypeError, match="weight must be"):
+        sd.fixed_dense_linear_cross_entropy(torch.zeros(3, 16), torch.zeros(3, dtype=torch.long), torch.zeros(8, 16, dtype=torch.int8), total=3)
