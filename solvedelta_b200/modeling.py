@@ -439,16 +439,17 @@ class SolveDeltaForCausalLM(SolveDeltaPreTrainedModel, GenerationMixin):
         inference on a CUDA device: half of their bytes in a cached token, twice the tensor rate in a prompt.  A short
         cached token is bound by launches, of which an int8 layer has more: one sequence at hidden size 1024 takes longer
         than in BF16 (194 against 175 us, six layers), at 2048 less (361 against 382).  The mixers stay in BF16.  In place,
-        not reversible; quantised modules are left as they are.  Checkpoints are those of the model before: quantise after
-        loading.  A head in int8 has no chunked loss: its logits are made whole.  Returns the model."""
+        not reversible; quantised modules are left as they are, a projection with hooks or adapters is refused (nothing is
+        changed then).  Checkpoints are those of the model before: quantise after loading.  A head in int8 has no chunked
+        loss: its logits are made whole.  Returns the model."""
         if head and self.config.tie_word_embeddings:
             raise ValueError("a tied head shares the embedding's weight and cannot be quantised")
-        for layer in self.model.layers:
-            for name in ("gate_up_proj", "down_proj"):
-                if not isinstance(getattr(layer.mlp, name), Int8Linear):
-                    setattr(layer.mlp, name, Int8Linear.from_linear(getattr(layer.mlp, name)))
-        if head and not isinstance(self.lm_head, Int8Linear):
-            self.lm_head = Int8Linear.from_linear(self.lm_head)
+        places = [(layer.mlp, name) for layer in self.model.layers for name in ("gate_up_proj", "down_proj")]
+        places += [(self, "lm_head")] if head else []
+        places = [(owner, name) for owner, name in places if not isinstance(getattr(owner, name), Int8Linear)]
+        made = [Int8Linear.from_linear(getattr(owner, name)) for owner, name in places]   # all of them, or an error and none
+        for (owner, name), projection in zip(places, made):
+            setattr(owner, name, projection)
         return self
 
     def _plain_head(self) -> bool:

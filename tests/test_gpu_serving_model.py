@@ -219,3 +219,19 @@ def test_quantised_models_of_odd_widths_decode(hidden, heads, rows):
         whole = model(input_ids=torch.cat((ids, ids[:, :1]), dim=1)).logits[:, -1].float()
         got = model(input_ids=ids[:, :1], past_key_values=step.past_key_values, use_cache=True).logits[:, -1].float()
     assert torch.isfinite(got).all() and ((got - whole).norm() / whole.norm()).item() < 0.1
+
+
+def test_a_model_is_quantised_as_a_whole_or_not_at_all():
+    model = _model()
+    last = model.model.layers[-1].mlp.down_proj
+    handle = last.register_forward_hook(lambda module, args, out: 2 * out)
+    with pytest.raises(TypeError, match="plain nn.Linear"):
+        model.quantize_int8(head=True)
+    assert not any(isinstance(module, sd.Int8Linear) for module in model.modules())
+    handle.remove()
+    model.quantize_int8()
+    assert sum(isinstance(module, sd.Int8Linear) for module in model.modules()) == 4
+    assert type(model.lm_head) is nn.Linear
+    kept = model.model.layers[0].mlp.gate_up_proj
+    model.quantize_int8(head=True)
+    assert isinstance(model.lm_head, sd.Int8Linear) and model.model.layers[0].mlp.gate_up_proj is kept
