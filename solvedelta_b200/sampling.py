@@ -26,8 +26,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: U
     temperature above 1e30 counts as 1e30.
 
     Logits of -inf and NaN are never drawn; those of +inf share the draw.  A row that has nothing to draw gets
-    ``empty_token``.  The weights are exact to 2^-45 of the largest and their sums are exact, so a row's token does not
-    depend on the batch it is in.  Nothing synchronises with the host: the call can be captured into a graph."""
+    ``empty_token``.  The weights are exact to 2^-45 of the largest (smaller ones are zero) and their sums are exact, so
+    a row's token does not depend on the batch it is in.  Nothing synchronises with the host: the call can be captured
+    into a graph."""
     return _lib.host().sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, int(empty_token))
 
 
